@@ -199,7 +199,7 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------------------------------------------
 def _act(z, act):
     if act == "relu":
-        return torch.where(z > 0, z, torch.zeros_like(z))
+        return torch.where(z < 0, torch.zeros_like(z), z)
     if act == "gelu":
         return 0.5 * z * (1.0 + torch.erf(z * math.sqrt(0.5)))
     if act == "gelu_tanh":
@@ -211,7 +211,7 @@ def _act(z, act):
 
 def _act_slope(z, act):
     if act == "relu":
-        return (z > 0).to(z.dtype)
+        return 1.0 - (z <= 0).to(z.dtype)
     if act == "gelu":
         return 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) * math.sqrt(0.5 / math.pi)
     if act == "gelu_tanh":
