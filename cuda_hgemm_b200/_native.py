@@ -24,6 +24,8 @@ EXPORTED_SYMBOLS = (
     "b200_hgemm_enable_multicast", "b200_hgemm_multicast_state", "b200_hgemm_plan_supported",
     "b200_hgemm_release_workspaces", "b200_hgemm_synchronize", "b200_hgemm_streamk_static_last_error",
     "b200_debug_wait_expiry_static", "b200_hgemm_fused_ex", "b200_hgemm_batched", "b200_hgemm_bkn", "b200_hgemm_host_a_after", "b200_sched_tile_coord_fast", "b200_debug_fast_div", "b200_debug_cluster_capacity",
+    "b200_hgemm_linear", "b200_hgemm_linear_workspace_bytes", "b200_hgemm_linear_backward", "b200_hgemm_grouped",
+    "b200_hgemm_grouped_backward", "b200_hgemm_backward_workspace_bytes",
 )
 
 OK = 0
@@ -48,6 +50,8 @@ VARIANT_HYBRID_PAIR = 8
 
 C_F16, C_BF16, C_F32 = 0, 1, 2
 
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
+
 MULTICAST_OFF, MULTICAST_ON, MULTICAST_LOCKED_OFF = 0, 1, 2
 
 
@@ -64,6 +68,18 @@ class Epilogue(Structure):
     """``b200_hgemm_epilogue``: C = alpha * A*B^T + beta * c_in + bias."""
     _fields_ = [("alpha", ctypes.c_float), ("beta", ctypes.c_float), ("bias", c_void_p), ("c_in", c_void_p),
                 ("c_type", c_int32)]
+
+
+class LinearArgs(Structure):
+    """``b200_linear_args``: C = act(A*B^T + bias) + residual."""
+    _fields_ = [("in_type", c_int32), ("c_type", c_int32), ("act", c_int32), ("bias", c_void_p), ("residual", c_void_p),
+                ("pre", c_void_p)]
+
+
+class LinearGrads(Structure):
+    """``b200_linear_grads``: what a backward pass reads and which gradients it writes."""
+    _fields_ = [("in_type", c_int32), ("c_type", c_int32), ("act", c_int32), ("db_type", c_int32), ("accumulate", c_int32),
+                ("dC", c_void_p), ("pre", c_void_p), ("dZ", c_void_p), ("dA", c_void_p), ("dB", c_void_p), ("dbias", c_void_p)]
 
 
 class HgemmError(RuntimeError):
@@ -100,6 +116,19 @@ def load() -> ctypes.CDLL:
     lib.b200_hgemm_fused_ex.restype = c_int
     lib.b200_hgemm_batched.argtypes = [c_void_p, c_void_p, c_void_p] + [c_size_t] * 7 + [c_void_p]
     lib.b200_hgemm_batched.restype = c_int
+    lib.b200_hgemm_linear.argtypes = [c_void_p] * 3 + [c_size_t] * 3 + [POINTER(LinearArgs), c_void_p, c_size_t, c_void_p]
+    lib.b200_hgemm_linear.restype = c_int
+    lib.b200_hgemm_linear_workspace_bytes.argtypes = [c_size_t] * 3 + [POINTER(LinearArgs)]
+    lib.b200_hgemm_linear_workspace_bytes.restype = c_size_t
+    lib.b200_hgemm_linear_backward.argtypes = [c_void_p] * 2 + [c_size_t] * 3 + [POINTER(LinearGrads), c_void_p, c_size_t, c_void_p]
+    lib.b200_hgemm_linear_backward.restype = c_int
+    lib.b200_hgemm_grouped.argtypes = [c_void_p] * 4 + [c_size_t] * 5 + [POINTER(LinearArgs), c_void_p]
+    lib.b200_hgemm_grouped.restype = c_int
+    lib.b200_hgemm_grouped_backward.argtypes = ([c_void_p] * 3 + [c_size_t] * 5 +
+                                                [POINTER(LinearGrads), c_void_p, c_size_t, c_void_p])
+    lib.b200_hgemm_grouped_backward.restype = c_int
+    lib.b200_hgemm_backward_workspace_bytes.argtypes = [c_size_t] * 4 + [POINTER(LinearGrads)]
+    lib.b200_hgemm_backward_workspace_bytes.restype = c_size_t
     lib.b200_hgemm_host.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t]
     lib.b200_hgemm_host.restype = c_int
     lib.b200_hgemm_host_a.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t]

@@ -17,6 +17,7 @@ from ._native import HgemmError, Plan, check
 
 __all__ = [
     "b200Hgemm", "b200HgemmCta1", "b200HgemmCta2", "b200HgemmSplitK", "b200HgemmStreamK", "b200HgemmSimt",
+    "hgemm_linear", "hgemm_linear_backward", "hgemm_grouped", "hgemm_grouped_backward", "ACTIVATIONS",
     "hgemm_ex", "hgemm_host", "select_plan", "workspace_bytes", "last_device_error", "launch_count",
     "KERNEL_LOG_NAMES", "Plan", "HgemmError",
 ]
@@ -175,6 +176,190 @@ def hgemm_batched(A, B, C):
         check(_native.load().b200_hgemm_batched(A.data_ptr(), B.data_ptr(), C.data_ptr(), int(M), int(N), int(K), int(batch),
                                                 int(A.stride(0)), int(stride_b), int(C.stride(0)), _stream_of(A)))
     return C
+
+
+# activation names of the feed-forward products -> B200_ACT_*
+ACTIVATIONS = {"none": _native.ACT_NONE, "relu": _native.ACT_RELU, "gelu": _native.ACT_GELU,
+               "gelu_tanh": _native.ACT_GELU_TANH, "silu": _native.ACT_SILU}
+
+
+def _type_code(dtype):
+    import torch
+
+    return {torch.float16: _native.C_F16, torch.bfloat16: _native.C_BF16, torch.float32: _native.C_F32}.get(dtype)
+
+
+def _act_code(act):
+    try:
+        return ACTIVATIONS[act]
+    except (KeyError, TypeError):
+        raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}") from None
+
+
+def _operand(name, t, dtypes, shape, device):
+    """A contiguous CUDA tensor of one of ``dtypes`` and of ``shape``; its address (``None`` for an absent one)."""
+    import torch
+
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or not t.is_cuda or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous CUDA tensor of type {' or '.join(str(d)[6:] for d in dtypes)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must live on {device}")
+    return t.data_ptr()
+
+
+def _rows_and_weights(A, B, offsets):
+    """Shapes and input type of ``A [M, K]`` and ``B [N, K]``, or ``B [G, N, K]`` where ``offsets`` are given."""
+    import torch
+
+    grouped = offsets is not None
+    for name, t, dims in (("A", A, 2), ("B", B, 3 if grouped else 2)):
+        if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float16, torch.bfloat16) or not t.is_cuda:
+            raise TypeError(f"{name} must be a float16 or bfloat16 CUDA tensor")
+        if t.dim() != dims:
+            raise ValueError(f"{name} must be {dims}-D")
+    if A.dtype != B.dtype:
+        raise TypeError("A and B must have one type")
+    if A.device != B.device:
+        raise ValueError("A and B must live on one device")
+    M, K = A.shape
+    N = B.shape[-2]
+    if B.shape[-1] != K:
+        raise ValueError(f"shape mismatch: A {tuple(A.shape)}, B {tuple(B.shape)}")
+    if not A.is_contiguous():
+        raise TypeError("A must be contiguous")
+    if not grouped:
+        if not B.is_contiguous():
+            raise TypeError("B must be contiguous")
+        return M, N, K, 1, N * K
+    G = B.shape[0]
+    # the matrices must be dense (a dimension of one element may have any stride); the stack may have gaps
+    if (B.stride(2) != 1 and K > 1) or (B.stride(1) != K and N > 1):
+        raise ValueError("the matrices of B must be contiguous")
+    if not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int32 or not offsets.is_cuda or not offsets.is_contiguous():
+        raise TypeError("offsets must be a contiguous int32 CUDA tensor")
+    if tuple(offsets.shape) != (G + 1,):
+        raise ValueError(f"offsets must have {G + 1} values, one more than B has matrices")
+    if offsets.device != A.device:
+        raise ValueError("offsets must live on A's device")
+    return M, N, K, G, B.stride(0) if G > 1 else N * K
+
+
+def _scratch(nbytes, device):
+    """Scratch memory of one call, from torch's caching allocator on the current stream (``None`` where none is needed)."""
+    import torch
+
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _linear_args(A, C, bias, act, residual, pre, bias_shape, M, N):
+    import torch
+
+    types = (A.dtype, torch.float32)
+    c_ptr = _operand("C", C, types, (M, N), A.device)
+    if c_ptr is None:
+        raise TypeError("C must be a CUDA tensor")
+    return c_ptr, _native.LinearArgs(
+        _type_code(A.dtype), _type_code(C.dtype), _act_code(act), _operand("bias", bias, (A.dtype,), bias_shape, A.device),
+        _operand("residual", residual, (C.dtype,), (M, N), A.device), _operand("pre", pre, (C.dtype,), (M, N), A.device))
+
+
+def hgemm_linear(A, B, C, bias=None, act: str = "none", residual=None, pre=None):
+    """``C = act(A @ B.T + bias) + residual`` in one kernel (C ABI ``b200_hgemm_linear``).
+
+    ``A [M, K]``, ``B [N, K]`` and ``bias [N]`` are float16 or bfloat16 (all of one type), ``C``, ``residual`` and ``pre``
+    ``[M, N]`` of that type or float32. ``act`` is one of ``ACTIVATIONS``. ``pre`` receives ``A @ B.T + bias``, which
+    :func:`hgemm_linear_backward` needs; ``residual`` may be ``C`` itself. ``K`` is a multiple of 8; ``M`` may be 0."""
+    import torch
+
+    M, N, K, _, _ = _rows_and_weights(A, B, None)
+    c_ptr, args = _linear_args(A, C, bias, act, residual, pre, (N,), M, N)
+    lib = _native.load()
+    with torch.cuda.device(A.device):
+        nbytes = lib.b200_hgemm_linear_workspace_bytes(M, N, K, ctypes.byref(args))
+        ws = _scratch(nbytes, A.device)
+        check(lib.b200_hgemm_linear(A.data_ptr(), B.data_ptr(), c_ptr, M, N, K, ctypes.byref(args),
+                                    ws.data_ptr() if ws is not None else None, nbytes, _stream_of(A)))
+    return C
+
+
+def hgemm_grouped(A, B, C, offsets, bias=None, act: str = "none", pre=None):
+    """Rows ``offsets[g] : offsets[g + 1]`` of ``C = act(those rows of A @ B[g].T + bias[g])``, for every group in one
+    launch (C ABI ``b200_hgemm_grouped``).
+
+    ``A [M, K]``, ``B [G, N, K]`` (dense matrices, any distance between them that is a multiple of 8 elements) and
+    ``bias [G, N]`` are float16 or bfloat16, ``C`` and ``pre`` ``[M, N]`` of that type or float32. ``offsets`` are ``G + 1``
+    ascending int32 values on the device, read there by the kernel: the host never needs the group sizes. Groups may
+    be empty; rows outside ``offsets[0] : offsets[G]`` are not written. ``K`` is a multiple of 8, ``G`` at most 1024."""
+    import torch
+
+    if offsets is None:
+        raise TypeError("offsets must be a contiguous int32 CUDA tensor")
+    M, N, K, G, stride = _rows_and_weights(A, B, offsets)
+    c_ptr, args = _linear_args(A, C, bias, act, None, pre, (G, N), M, N)
+    with torch.cuda.device(A.device):
+        check(_native.load().b200_hgemm_grouped(A.data_ptr(), B.data_ptr(), c_ptr, offsets.data_ptr(), M, N, K, G, stride,
+                                                ctypes.byref(args), _stream_of(A)))
+    return C
+
+
+def _backward(dC, A, B, offsets, act, pre, dA, dB, dbias, dZ, accumulate):
+    import torch
+
+    M, N, K, G, stride = _rows_and_weights(A, B, offsets)
+    dtype, device = A.dtype, A.device
+    if not isinstance(dC, torch.Tensor):
+        raise TypeError("dC must be a CUDA tensor")
+    dc_ptr = _operand("dC", dC, (dtype, torch.float32), (M, N), device)
+    stack = (G,) if offsets is not None else ()
+    code = _act_code(act)
+    if code != _native.ACT_NONE and pre is None:
+        raise ValueError("the gradient of an activation needs pre, the value before it")
+    if dA is None and dB is None and dbias is None and dZ is None:
+        raise ValueError("none of dA, dB, dbias and dZ was asked for")
+    grads = _native.LinearGrads(
+        _type_code(dtype), _type_code(dC.dtype), code, _type_code(dB.dtype) if isinstance(dB, torch.Tensor) else _type_code(dtype),
+        1 if accumulate else 0, dc_ptr, _operand("pre", pre, (dC.dtype,), (M, N), device),
+        _operand("dZ", dZ, (dtype,), (M, N), device), _operand("dA", dA, (dtype,), (M, K), device),
+        _operand("dB", dB, (dtype, torch.float32), stack + (N, K), device),
+        _operand("dbias", dbias, (torch.float32,), stack + (N,), device))
+    lib = _native.load()
+    with torch.cuda.device(device):
+        nbytes = lib.b200_hgemm_backward_workspace_bytes(M, N, K, G, ctypes.byref(grads))
+        ws = _scratch(nbytes, device)
+        ws_ptr = ws.data_ptr() if ws is not None else None
+        if offsets is None:
+            check(lib.b200_hgemm_linear_backward(A.data_ptr(), B.data_ptr(), M, N, K, ctypes.byref(grads), ws_ptr, nbytes,
+                                                 _stream_of(A)))
+        else:
+            check(lib.b200_hgemm_grouped_backward(A.data_ptr(), B.data_ptr(), offsets.data_ptr(), M, N, K, G, stride,
+                                                  ctypes.byref(grads), ws_ptr, nbytes, _stream_of(A)))
+
+
+def hgemm_linear_backward(dC, A, B, act: str = "none", pre=None, dA=None, dB=None, dbias=None, dZ=None, accumulate: bool = False):
+    """The gradients of :func:`hgemm_linear` that are asked for (C ABI ``b200_hgemm_linear_backward``): with
+    ``dZ = dC * act'(pre)``, ``dA = dZ @ B``, ``dB = dZ.T @ A`` and ``dbias`` the column sums of ``dZ``.
+
+    ``dC`` and ``pre`` ``[M, N]`` have the forward pass's C type; ``dA [M, K]`` and ``dZ [M, N]`` the inputs' type, ``dB [N, K]``
+    that type or float32, ``dbias [N]`` float32 (summed before ``dZ`` is rounded for the products). With ``accumulate``
+    the new ``dB`` (float32 then) and ``dbias`` are added to what the tensors hold. The gradient of the residual is
+    ``dC``. ``N`` and ``K`` are multiples of 8; ``M`` may be 0. Returns ``(dA, dB, dbias)``."""
+    _backward(dC, A, B, None, act, pre, dA, dB, dbias, dZ, accumulate)
+    return dA, dB, dbias
+
+
+def hgemm_grouped_backward(dC, A, B, offsets, act: str = "none", pre=None, dA=None, dB=None, dbias=None, dZ=None,
+                           accumulate: bool = False):
+    """The gradients of :func:`hgemm_grouped` (C ABI ``b200_hgemm_grouped_backward``), as
+    :func:`hgemm_linear_backward` group by group: ``dB [G, N, K]``, ``dbias [G, N]``. A group without rows gets zeros; rows of
+    ``dA`` and ``dZ`` outside every group are not written."""
+    if offsets is None:
+        raise TypeError("offsets must be a contiguous int32 CUDA tensor")
+    _backward(dC, A, B, offsets, act, pre, dA, dB, dbias, dZ, accumulate)
+    return dA, dB, dbias
 
 
 def hgemm_host(A_host, B_host, C_host):

@@ -48,7 +48,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         return LIB_SO
     LIB_DIR.mkdir(exist_ok=True)
     cmd = [nvcc(), *COMMON_FLAGS, "--shared", "-Xcompiler", "-fPIC", "-cudart", "static",
-           "-o", str(LIB_SO), *[str(s) for s in sorted(CSRC.glob("*.cu"))]]
+           "-o", str(LIB_SO), "--split-compile", "0", *[str(s) for s in sorted(CSRC.glob("*.cu"))]]
     if verbose:
         cmd.insert(1, "-Xptxas")
         cmd.insert(2, "-v")

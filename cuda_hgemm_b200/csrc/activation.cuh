@@ -1,0 +1,121 @@
+// The activations of a feed-forward layer and their slopes, in FP32, for epilogues and the pass that
+// multiplies an output's gradient by the slope.
+//
+//   relu       max(z, 0)                              slope  z > 0
+//   gelu       z Phi(z), Phi(z) = (1 + erf(z/sqrt 2))/2   slope  Phi(z) + z exp(-z^2/2)/sqrt(2 pi)
+//   gelu_tanh  z s, s = 1/(1 + exp(-w)), w = 2 sqrt(2/pi) (z + 0.044715 z^3)   slope  s + z s (1-s) w'
+//   silu       z s, s = 1/(1 + exp(-z))               slope  s + z s (1-s)
+//
+// (0.5 (1 + tanh(w/2)) is that s: one exponential and one division instead of a tanh.) A NaN stays a NaN.
+// Where s (1-s) has underflown, z is held at a bound before it multiplies it, so that a large z gives the
+// slope 0 or 1 and not 0 * infinity.
+#pragma once
+
+#include <stdint.h>
+
+namespace b200 {
+
+// The values of B200_ACT_* in the public header.
+enum ActKind : uint32_t {
+    kActNone = 0,
+    kActRelu = 1,
+    kActGelu = 2,
+    kActGeluTanh = 3,
+    kActSilu = 4,
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGeluTanhScale = 1.5957691216057308f;  // 2 sqrt(2/pi)
+constexpr float kGeluTanhCubic = 0.044715f;
+
+// 2^x by the hardware's approximation (relative error about 2^-22, 0 and infinity at the ends).
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// z held within [-bound, bound]; a NaN stays
+__device__ __forceinline__ float held(float z, float bound) {
+    return z > bound ? bound : (z < -bound ? -bound : z);
+}
+
+// 1 - Phi(|z|) and exp(-z^2/2): erfc(x) = t (a1 + t (a2 + ... a5)) exp(-x^2) with t = 1/(1 + p x), x = |z|/sqrt 2
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: absolute error below 1.5e-7, so Phi is off by
+// less than 1e-7). No branch, and about half the instructions of erff, which the epilogue warps would feel.
+__device__ __forceinline__ float normal_tail(float z, float *gauss) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    float poly = fmaf(1.061405429f, t, -1.453152027f);
+    poly = fmaf(poly, t, 1.421413741f);
+    poly = fmaf(poly, t, -0.284496736f);
+    poly = fmaf(poly, t, 0.254829592f);
+    *gauss = exp2_approx(-kLog2e * x * x);
+    return 0.5f * poly * t * *gauss;
+}
+
+// 1 / (1 + exp(-z (a + b z^2))): silu's gate with a = 1, b = 0, that of gelu_tanh with the two constants above.
+__device__ __forceinline__ float logistic_gate(float z, float a, float b) {
+    return __fdividef(1.f, 1.f + exp2_approx(-kLog2e * z * fmaf(b * z, z, a)));
+}
+
+template <uint32_t KIND>
+__device__ __forceinline__ float act_value(float z) {
+    if (KIND == kActRelu) return z < 0.f ? 0.f : z;
+    if (KIND == kActGelu) {
+        float gauss;
+        const float tail = normal_tail(z, &gauss);
+        return z * (z < 0.f ? tail : 1.f - tail);
+    }
+    if (KIND == kActGeluTanh) return z * logistic_gate(z, kGeluTanhScale, kGeluTanhScale * kGeluTanhCubic);
+    if (KIND == kActSilu) return z * logistic_gate(z, 1.f, 0.f);
+    return z;
+}
+
+template <uint32_t KIND>
+__device__ __forceinline__ float act_slope(float z) {
+    if (KIND == kActRelu) return z <= 0.f ? 0.f : 1.f;
+    if (KIND == kActGelu) {
+        const float h = held(z, 16.f);  // exp(-128): gone
+        float gauss;
+        const float tail = normal_tail(h, &gauss);
+        return (h < 0.f ? tail : 1.f - tail) + h * 0.3989422804014327f * gauss;
+    }
+    if (KIND == kActGeluTanh) {
+        const float h = held(z, 16.f);
+        const float s = logistic_gate(h, kGeluTanhScale, kGeluTanhScale * kGeluTanhCubic);
+        return s + h * s * (1.f - s) * kGeluTanhScale * fmaf(3.f * kGeluTanhCubic * h, h, 1.f);
+    }
+    if (KIND == kActSilu) {
+        const float h = held(z, 80.f);  // exp(80) is still finite
+        const float s = logistic_gate(h, 1.f, 0.f);
+        return s + h * s * (1.f - s);
+    }
+    return 1.f;
+}
+
+// COUNT values (FP32 bit patterns) through one activation; the choice is made once, outside the loop.
+template <int COUNT, uint32_t KIND>
+__device__ __forceinline__ void act_apply_kind(uint32_t *vals) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) vals[j] = __float_as_uint(act_value<KIND>(__uint_as_float(vals[j])));
+}
+
+template <int COUNT>
+__device__ __forceinline__ void act_apply(uint32_t *vals, uint32_t kind) {
+    if (kind == kActGeluTanh || kind == kActSilu) {
+        // one loop for both: the gates differ in two constants
+        const float a = kind == kActSilu ? 1.f : kGeluTanhScale, b = kind == kActSilu ? 0.f : kGeluTanhScale * kGeluTanhCubic;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            const float z = __uint_as_float(vals[j]);
+            vals[j] = __float_as_uint(z * logistic_gate(z, a, b));
+        }
+    } else if (kind == kActGelu) {
+        act_apply_kind<COUNT, kActGelu>(vals);
+    } else if (kind == kActRelu) {
+        act_apply_kind<COUNT, kActRelu>(vals);
+    }
+}
+
+}  // namespace b200

@@ -1,0 +1,667 @@
+// Products over ragged groups of rows: the feed-forward products of a layer whose rows were sorted by expert,
+// and, with a single group, those of a dense layer. Three forms of one kernel, with A [T x K], B_g [N x K],
+// C [T x N] and the rows [offsets[g], offsets[g+1]) belonging to group g:
+//
+//   kFormForward  C[t][n]    = act(sum_k A[t][k] B_g[n][k] + bias_g[n])   rows of group g
+//   kFormInput    dA[t][k]   = sum_n dC[t][n] B_g[n][k]                   rows of group g
+//   kFormWeight   dB_g[n][k] = sum_t dC[t][n] A[t][k]                     t over the rows of group g
+//
+// The MMA's row operand is called P here and its column operand Q. Forward and input gradient put the weights
+// on P (n, or k) and the rows of the group on Q, so the accumulator holds the result transposed: tensor-memory
+// lane = output column, tensor-memory column = row of the group. An MMA's column count is chosen at run
+// time in steps of 16 (32 for a pair), so a group of 300 rows is two blocks of 160 and 140, where the other
+// way round it would be three blocks of 128 (or two of 256 on a pair) filled to 78 (59) percent; a group of three
+// rows costs an MMA of 16 columns and stages 16 rows. The rows' operand is staged by at most four copies out of
+// boxes of 128, 64, 32 and 16 rows. The weight gradient sums over the group's rows: both operands
+// are then row-contiguous in the other index and read by the MMA as MN-major; the accumulator is not transposed.
+//
+// Group sizes are known on the device only (a router wrote them): every CTA reads the offsets, cuts the groups
+// into tiles and walks its share of them. Offsets that are out of order or past T are held within [0, T].
+//
+// A block of rows that reaches past its group's end reads rows of the next group. For P and Q of the first two
+// forms this only adds accumulator columns that are never stored. In the weight gradient those rows are
+// summed over: the lines of the last block behind the group's end (a row of a box is one 128-byte line) are
+// overwritten with zeros in both operands before the MMA reads them, so that whatever the next group holds, NaN
+// included, stays out of the sum.
+//
+// Warp roles, ring, accumulators and bounded waits are those of hgemm_tcgen05_kernel (gemm_kernel.cuh); the
+// reference has no counterpart (one product per launch, src/main.cu:11).
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "activation.cuh"
+#include "ptx_sm100.cuh"
+#include "sched.h"
+
+namespace b200 {
+
+enum GroupedForm : int {
+    kFormForward = 0,
+    kFormInput = 1,
+    kFormWeight = 2,
+};
+
+constexpr int kGroupedThreads = 192;
+constexpr uint32_t kGroupedMaxGroups = 1024;
+constexpr uint32_t kGroupedBand = 8;  // blocks of rows a band of tiles is high
+
+struct alignas(64) GroupedParams {
+    CUtensorMap tm_p;     // forward {K, N, groups} box {64, 128}; input {K, N, groups} box {64, 64}; weight {N, T} box {64, 64}
+    CUtensorMap tm_q[4];  // forward {K, T}, input {N, T}: boxes {64, 128 >> i}; weight: [0] = {K, T} box {64, 64}
+    CUtensorMap tm_out;   // weight: {K, N, groups}, box of 128 bytes x 32 rows
+    void *out;
+    void *pre;             // forward: Z = sum + bias before the activation, or null
+    const void *bias;      // forward: groups x N of the inputs' type, or null
+    const int32_t *offsets;  // groups + 1, or null: one group of all rows
+    uint32_t *error_word;
+    uint32_t rows;         // T
+    uint32_t groups;
+    uint32_t p_dim;        // extent on P: N, K, N
+    uint32_t q_dim;        // weight: K
+    uint32_t k_blocks;     // forward, input: stages of the summed index
+    uint32_t q_max;        // forward, input: most rows of a block
+    uint32_t p_blocks;
+    uint32_t q_blocks;     // weight
+    uint32_t in_bf16;
+    uint32_t out_type;     // 0 FP16, 1 BF16, 2 FP32
+    uint32_t act;
+    uint32_t accumulate;   // weight, FP32: add to the output
+    FastDiv p_div;         // by p_blocks
+};
+
+template <int FORM, int CG, int QT, int STAGES, int KPS>
+struct GroupedTraits {
+    static constexpr bool kWeight = FORM == kFormWeight;
+    static_assert(CG == 1 || CG == 2, "single CTAs or CTA pairs");
+    static_assert(QT == 32 || QT == 64 || QT == 128 || QT == 256, "columns of an accumulator");
+    static_assert(!kWeight || (QT / CG == 128 && KPS == 1), "weight form: two 64-column boxes of Q per CTA");
+    static constexpr uint32_t kStep = 16u * CG;  // an MMA's columns come in these steps
+    static constexpr uint32_t kPBytes = 128u * 128u;
+    static constexpr uint32_t kQBytes = (QT / CG) * 128u;
+    static constexpr uint32_t kBlockBytes = kPBytes + kQBytes;
+    static constexpr uint32_t kStageBytes = KPS * kBlockBytes;
+    static constexpr uint32_t kTmemCols = 2u * QT;
+    static constexpr uint32_t kStagingBytes = kWeight ? 4u * 2u * 4096u : 0u;
+    static constexpr uint32_t kTableBytes = kWeight ? 0u : 2u * 4u * (kGroupedMaxGroups + 4u);
+    static constexpr uint32_t kBarrierBytes = 256;
+    static constexpr uint32_t kSmemBytes = 1024 + STAGES * kStageBytes + kStagingBytes + kTableBytes + kBarrierBytes;
+    static_assert(kBlockBytes % 1024 == 0, "operand slabs must keep 1024-byte alignment");
+    static_assert(kSmemBytes <= 232448, "exceeds 227 KB of shared memory");
+    static_assert((kWeight ? 32u : 16u) * STAGES + 40u <= kBarrierBytes, "barrier area too small");
+    static_assert(QT / CG <= 128, "rows of Q a CTA stages: one box of 128 and the smaller ones");
+    static_assert(STAGES <= 16, "one lane of a warp per barrier to set up");
+};
+
+// One piece of work: an output tile and, in the weight form, the rows it sums over.
+struct GroupedTile {
+    uint32_t group;
+    uint32_t p0;     // first index on P of the whole tile (of the pair)
+    uint32_t q0;     // forward, input: first row; weight: first index on Q
+    uint32_t valid;  // forward, input: rows stored; weight: rows summed over
+    uint32_t n_mma;  // columns of the MMA
+    uint32_t row0;   // weight: first row of the group
+};
+
+__device__ __forceinline__ uint32_t round_up_u32(uint32_t v, uint32_t step) {
+    return (v + step - 1u) / step * step;
+}
+
+// Rows of a group as the offsets say, held within [0, T].
+__device__ __forceinline__ uint32_t held_offset(int32_t v, uint32_t rows) {
+    return v < 0 ? 0u : min(static_cast<uint32_t>(v), rows);
+}
+
+// Block index inside a group -> (block on Q, block on P): bands of kGroupedBand blocks of rows, the row block
+// moving fastest, so that the tiles that run at one time share the weights of a few P blocks and the rows
+// of at most eight Q blocks; odd bands walk P backwards.
+__device__ __forceinline__ void band_coord(uint32_t local, uint32_t nq, uint32_t np, uint32_t *q, uint32_t *p) {
+    if (nq == 1) {
+        *q = 0;
+        *p = local;
+        return;
+    }
+    const uint32_t per_band = kGroupedBand * np;
+    const uint32_t band = local / per_band;
+    const uint32_t rem = local - band * per_band;
+    const uint32_t high = min(kGroupedBand, nq - band * kGroupedBand);
+    const uint32_t pi = rem / high;
+    *q = band * kGroupedBand + (rem - pi * high);
+    *p = (band & 1u) ? np - 1u - pi : pi;
+}
+
+// Forward and input form: tile id -> tile. off / cum: the table of offsets and of row blocks before each group.
+template <int CG>
+__device__ __forceinline__ void rows_tile(const GroupedParams &p, const uint32_t *off, const uint32_t *cum, uint32_t t,
+                                          GroupedTile &out) {
+    const uint32_t block = fast_div(t, p.p_div);
+    uint32_t lo = 0, hi = p.groups;  // the largest g with cum[g] <= block; cum[groups] > block
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (cum[mid] <= block) lo = mid; else hi = mid;
+    }
+    const uint32_t first = cum[lo], nq = cum[lo + 1u] - first;
+    const uint32_t start = off[lo], end = max(off[lo + 1u], start), r = end - start;
+    uint32_t qb, pb;
+    band_coord(t - first * p.p_blocks, nq, p.p_blocks, &qb, &pb);
+    const uint32_t size = round_up_u32((r + nq - 1u) / nq, 16u * CG);  // even blocks
+    out.group = lo;
+    out.p0 = pb * 128u * CG;
+    out.q0 = start + qb * size;
+    out.valid = min(size, r - qb * size);
+    out.n_mma = round_up_u32(out.valid, 16u * CG);
+    out.row0 = 0;
+}
+
+// Weight form: tile id -> tile (the same number of tiles for every group).
+template <int CG, int QT>
+__device__ __forceinline__ void weight_tile(const GroupedParams &p, uint32_t t, GroupedTile &out) {
+    const uint32_t per_group = p.p_blocks * p.q_blocks;
+    const uint32_t g = t / per_group;
+    uint32_t qb, pb;
+    band_coord(t - g * per_group, p.q_blocks, p.p_blocks, &qb, &pb);
+    uint32_t start = 0, end = p.rows;
+    if (p.offsets) {
+        start = held_offset(__ldg(p.offsets + g), p.rows);
+        end = max(held_offset(__ldg(p.offsets + g + 1), p.rows), start);
+    }
+    out.group = g;
+    out.p0 = pb * 128u * CG;
+    out.q0 = qb * QT;
+    out.valid = end - start;
+    out.n_mma = min(static_cast<uint32_t>(QT), round_up_u32(p.q_dim - out.q0, 16u * CG));
+    out.row0 = start;
+}
+
+// An mbarrier wait that also acquires what other CTAs of the cluster wrote before they arrived.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t"
+        "}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+__device__ __forceinline__ uint32_t pack2_typed(uint32_t lo_f32_bits, uint32_t hi_f32_bits, uint32_t bf16) {
+    if (bf16) {
+        __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(lo_f32_bits), __uint_as_float(hi_f32_bits));
+        return *reinterpret_cast<uint32_t *>(&b);
+    }
+    return pack_half2_rn(lo_f32_bits, hi_f32_bits);
+}
+
+// A 32-column chunk of a transposed accumulator (this lane: output column `col`, register j: row q0 + j) to
+// row-major memory. 16-bit outputs whose rows are a whole number of 4-byte words leave two columns at a
+// time: neighbouring lanes exchange halves, the even lane takes the even rows and the odd lane the odd rows,
+// so that a warp stores two rows of 64 bytes with one instruction instead of one.
+__device__ __forceinline__ void store_transposed32(void *out, uint32_t out_type, uint32_t q0, uint32_t valid, uint32_t col,
+                                                   uint32_t dim, const uint32_t (&r)[32], uint32_t lane) {
+    if (out_type == 2u) {
+        float *dst = static_cast<float *>(out) + static_cast<size_t>(q0) * dim + col;
+#pragma unroll
+        for (uint32_t j = 0; j < 32; ++j) {
+            if (j < valid && col < dim) dst[static_cast<size_t>(j) * dim] = __uint_as_float(r[j]);
+        }
+        return;
+    }
+    if ((dim & 1u) == 0) {
+        const uint32_t odd = lane & 1u;
+        uint32_t *dst = static_cast<uint32_t *>(out) + ((static_cast<size_t>(q0) + odd) * dim + (col & ~1u)) / 2u;
+#pragma unroll
+        for (uint32_t j = 0; j < 32; j += 2) {
+            const uint32_t mine = pack2_typed(r[j], r[j + 1], out_type);  // rows j and j + 1 of this column
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+            // even lane: row j of (this, next) column; odd lane: row j + 1 of (previous, this)
+            const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+            if (j + odd < valid && col < dim) dst[static_cast<size_t>(j) * (dim / 2u)] = word;
+        }
+        return;
+    }
+    unsigned short *dst = static_cast<unsigned short *>(out) + static_cast<size_t>(q0) * dim + col;
+#pragma unroll
+    for (uint32_t j = 0; j < 32; ++j) {
+        if (j < valid && col < dim) dst[static_cast<size_t>(j) * dim] = static_cast<unsigned short>(pack2_typed(r[j], r[j], out_type));
+    }
+}
+
+template <int FORM, int CG, int QT, int STAGES, int KPS>
+__global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const __grid_constant__ GroupedParams p) {
+    using T = GroupedTraits<FORM, CG, QT, STAGES, KPS>;
+    constexpr bool WEIGHT = FORM == kFormWeight;
+    constexpr bool P_MN = FORM != kFormForward;  // P is read MN-major
+    constexpr uint32_t kStepK = 64u;             // summed index per k-block
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    const uint32_t base = (raw_addr + 1023u) & ~1023u;
+    uint8_t *base_ptr = smem_raw + (base - raw_addr);
+    const uint32_t staging = base + STAGES * T::kStageBytes;
+    uint8_t *staging_ptr = base_ptr + STAGES * T::kStageBytes;
+    uint32_t *off = reinterpret_cast<uint32_t *>(staging_ptr + T::kStagingBytes);
+    uint32_t *cum = off + kGroupedMaxGroups + 4u;
+    const uint32_t bars = staging + T::kStagingBytes + T::kTableBytes;
+    uint8_t *bars_ptr = staging_ptr + T::kStagingBytes + T::kTableBytes;
+    // full[STAGES] | empty[STAGES] | tmem_full[2] | tmem_empty[2] | tmem base | abort | tail_full[STAGES] | tail_ready[STAGES]
+    const uint32_t full_bar = bars;
+    const uint32_t empty_bar = bars + 8u * STAGES;
+    const uint32_t tfull_bar = bars + 16u * STAGES;
+    const uint32_t tempty_bar = tfull_bar + 16u;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars_ptr + 16u * STAGES + 32u);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    // pairs in the weight form: a stage that holds a tail has landed in this CTA / has been cleared in both CTAs. One of
+    // each per stage: several tails may be in the ring at once, and a stage is armed again only after its MMAs.
+    const uint32_t tail_bar = tfull_bar + 40u;
+    const uint32_t ready_bar = tail_bar + 8u * STAGES;
+
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t cta_rank = (CG == 2) ? cluster_cta_rank() : 0u;
+    const uint32_t worker = blockIdx.x / CG;
+    const uint32_t workers = gridDim.x / CG;
+
+    if (warp == 0) {
+        if (lane < static_cast<uint32_t>(STAGES)) {
+            mbar_init(full_bar + 8u * lane, 1);
+            mbar_init(empty_bar + 8u * lane, 1);
+        } else if (lane < static_cast<uint32_t>(STAGES) + 2u) {
+            const uint32_t a = lane - STAGES;
+            mbar_init(tfull_bar + 8u * a, 1);
+            mbar_init(tempty_bar + 8u * a, 4 * CG);
+        } else if (lane == static_cast<uint32_t>(STAGES) + 2u) {
+            *abort_flag = 0;
+        }
+        if (WEIGHT && CG == 2 && lane < static_cast<uint32_t>(STAGES)) {
+            mbar_init(tail_bar + 8u * lane, 1);
+            mbar_init(ready_bar + 8u * lane, 2);  // the MMA warps of both CTAs
+        }
+        fence_mbar_init();
+        __syncwarp();
+    }
+    if (warp == 2 && lane == 0) {
+        tma_prefetch_desc(&p.tm_p);
+        tma_prefetch_desc(&p.tm_q[0]);
+        if (WEIGHT) tma_prefetch_desc(&p.tm_out);
+    }
+    if (warp == 1) {
+        tmem_alloc<CG>(smem_u32(const_cast<uint32_t *>(tmem_slot)), T::kTmemCols);
+        tmem_relinquish<CG>();
+    }
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();  // offsets and operands may have been written, and outputs read, by the previous kernel
+
+    uint32_t tiles;
+    if (WEIGHT) {
+        tiles = p.groups * p.p_blocks * p.q_blocks;
+    } else {
+        for (uint32_t g = threadIdx.x; g <= p.groups; g += kGroupedThreads) {
+            off[g] = p.offsets ? held_offset(__ldg(p.offsets + g), p.rows) : (g == 0 ? 0u : p.rows);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            // blocks of at most q_max rows before each group: a running sum over 32 groups at a time
+            uint32_t total = 0;
+            for (uint32_t g0 = 0; g0 < p.groups; g0 += 32u) {
+                const uint32_t g = g0 + lane;
+                uint32_t blocks = 0;
+                if (g < p.groups) {
+                    const uint32_t start = off[g], end = max(off[g + 1u], start);
+                    blocks = (end - start + p.q_max - 1u) / p.q_max;
+                }
+                uint32_t sum = blocks;
+#pragma unroll
+                for (uint32_t d = 1; d < 32; d <<= 1) {
+                    const uint32_t up = __shfl_up_sync(0xffffffffu, sum, d);
+                    if (lane >= d) sum += up;
+                }
+                if (g < p.groups) cum[g] = total + sum - blocks;
+                total += __shfl_sync(0xffffffffu, sum, 31);
+            }
+            if (lane == 0) cum[p.groups] = total;
+        }
+    }
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();  // the peer's copies and arrivals target this CTA's barriers
+    tcgen05_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    if (!WEIGHT) tiles = cum[p.groups] * p.p_blocks;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (uint32_t t = worker; ok && t < tiles; t += workers) {
+                GroupedTile tile;
+                if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
+                const uint32_t blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks;
+                const uint32_t q_rows = tile.n_mma / CG;  // forward, input: rows this CTA stages
+                const int32_t p_at = static_cast<int32_t>(tile.p0 + cta_rank * 128u);
+                const int32_t q_at = static_cast<int32_t>(tile.q0 + cta_rank * q_rows);
+                const uint32_t bytes = KPS * (T::kPBytes + (WEIGHT ? T::kQBytes : q_rows * 128u));
+                for (uint32_t kb = 0; kb < blocks; ++kb) {
+                    if (!mbar_wait(empty_bar + 8u * stage, phase ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t slot = base + stage * T::kStageBytes;
+                    // the last block of a group that does not fill it: its lines are cleared behind the group's end
+                    const bool tail = WEIGHT && kb + 1u == blocks && (tile.valid & (kStepK - 1u)) != 0;
+                    // A pair's copies complete on the leader's barrier, which expects the bytes of both; a tail's on
+                    // the barrier of the CTA whose MMA warp clears its part.
+                    const bool pair = CG == 2 && !tail;
+                    uint32_t bar = full_bar + 8u * stage;
+                    if (CG == 2 && tail) {
+                        if (cta_rank == 0) mbar_arrive(bar);  // keeps the stage's phase; nothing is waited for there
+                        bar = tail_bar + 8u * stage;
+                        mbar_arrive_expect_tx(bar, bytes);
+                    } else if (CG == 2) {
+                        if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2u * bytes);
+                        bar = map_to_cta(bar, 0);
+                    } else {
+                        mbar_arrive_expect_tx(bar, bytes);
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < KPS; ++j) {
+                        const uint32_t sp = slot + j * T::kBlockBytes;
+                        const uint32_t sq = sp + T::kPBytes;
+                        const int32_t kx = static_cast<int32_t>((kb * KPS + j) * kStepK);  // past the end: zeros in both operands
+                        if (WEIGHT) {
+                            const int32_t row = static_cast<int32_t>(tile.row0) + kx;
+#pragma unroll
+                            for (int32_t h = 0; h < 2; ++h) {
+                                if (pair) {
+                                    tma_load_2d_pair(sp + h * 8192u, &p.tm_p, p_at + h * 64, row, bar);
+                                    tma_load_2d_pair(sq + h * 8192u, &p.tm_q[0], q_at + h * 64, row, bar);
+                                } else {
+                                    tma_load_2d(sp + h * 8192u, &p.tm_p, p_at + h * 64, row, bar);
+                                    tma_load_2d(sq + h * 8192u, &p.tm_q[0], q_at + h * 64, row, bar);
+                                }
+                            }
+                        } else {
+                            const int32_t g = static_cast<int32_t>(tile.group);
+                            if (FORM == kFormForward) {
+                                if (pair) tma_load_3d_pair(sp, &p.tm_p, kx, p_at, g, bar); else tma_load_3d(sp, &p.tm_p, kx, p_at, g, bar);
+                            } else {
+#pragma unroll
+                                for (int32_t h = 0; h < 2; ++h) {
+                                    if (pair) tma_load_3d_pair(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
+                                    else tma_load_3d(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
+                                }
+                            }
+                            uint32_t done = 0;
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) {
+                                const uint32_t box = 128u >> i;
+                                if (box <= static_cast<uint32_t>(QT / CG) && q_rows - done >= box) {
+                                    const int32_t y = q_at + static_cast<int32_t>(done);
+                                    if (pair) tma_load_2d_pair(sq + done * 128u, &p.tm_q[i], kx, y, bar);
+                                    else tma_load_2d(sq + done * 128u, &p.tm_q[i], kx, y, bar);
+                                    done += box;
+                                }
+                            }
+                        }
+                    }
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        // The whole warp walks the tiles; one lane of the leader issues. In the weight form all lanes clear the lines
+        // of a tail (in both CTAs of a pair).
+        if (cta_rank == 0 || WEIGHT) {
+            const uint32_t idesc_base = umma_idesc_f16_f32(128 * CG, 0) | (P_MN ? kUmmaIdescAMn : 0u) | (WEIGHT ? (1u << 16) : 0u) |
+                                        (p.in_bf16 ? kUmmaIdescBf16 : 0u);
+            uint32_t stage = 0, phase = 0, it = 0;
+            uint32_t tail_phase = 0;  // bit s: parity of stage s's next tail
+            bool ok = true;
+            for (uint32_t t = worker; ok && t < tiles; t += workers) {
+                GroupedTile tile;
+                if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
+                const uint32_t blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks;
+                if (blocks == 0) continue;
+                const uint32_t rest = WEIGHT ? (tile.valid & (kStepK - 1u)) : 0u;  // rows of a tail, 0: whole blocks
+                const uint32_t acc = it & 1u;
+                const uint32_t d_tmem = tmem_base + acc * QT;
+                const uint32_t idesc = idesc_base | ((tile.n_mma >> 3) << 17);
+                if (cta_rank == 0 && lane == 0) {
+                    if (!mbar_wait(tempty_bar + 8u * acc, ((it >> 1) & 1u) ^ 1u, abort_flag)) ok = false;
+                    tcgen05_fence_after_sync();
+                    const uint32_t whole = blocks - (rest != 0 ? 1u : 0u);
+                    for (uint32_t kb = 0; ok && kb < whole; ++kb) {
+                        if (!mbar_wait(full_bar + 8u * stage, phase, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tcgen05_fence_after_sync();
+                        const uint32_t slot = base + stage * T::kStageBytes;
+#pragma unroll
+                        for (uint32_t j = 0; j < KPS; ++j) {
+                            const uint32_t sp = slot + j * T::kBlockBytes, sq = sp + T::kPBytes;
+                            const uint64_t dp = P_MN ? umma_smem_desc_sw128_mn(sp, 8192u) : umma_smem_desc_sw128(sp);
+                            const uint64_t dq = WEIGHT ? umma_smem_desc_sw128_mn(sq, 8192u) : umma_smem_desc_sw128(sq);
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                umma_f16<CG>(d_tmem, dp + (P_MN ? 128u : 2u) * k, dq + (WEIGHT ? 128u : 2u) * k, idesc,
+                                             (kb > 0 || j > 0 || k > 0) ? 1u : 0u);
+                            }
+                        }
+                        if (CG == 1) umma_commit(empty_bar + 8u * stage); else umma_commit_pair(empty_bar + 8u * stage, 0x3);
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                if constexpr (WEIGHT) {
+                    // every lane follows: where the ring stands, and whether to go on
+                    ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                    if (CG == 2 && cta_rank != 0) {
+                        const uint32_t at = stage + blocks - (rest != 0 ? 1u : 0u);
+                        stage = at % STAGES;
+                        phase ^= (at / STAGES) & 1u;
+                    } else {
+                        stage = __shfl_sync(0xffffffffu, stage, 0);
+                        phase = __shfl_sync(0xffffffffu, phase, 0);
+                    }
+                    if (ok && rest != 0) {
+                        const uint32_t slot = base + stage * T::kStageBytes;
+                        const uint32_t landed_bar = (CG == 2 ? tail_bar : full_bar) + 8u * stage;
+                        const uint32_t parity = CG == 2 ? (tail_phase >> stage) & 1u : phase;
+                        uint32_t landed = 1;
+                        if (lane == 0) landed = mbar_wait(landed_bar, parity, abort_flag) ? 1u : 0u;
+                        landed = __shfl_sync(0xffffffffu, landed, 0);
+                        if (landed) {
+                            // each lane passes the completed barrier itself: the copies' bytes are then ordered before its stores
+                            mbar_try_wait(landed_bar, parity);
+                            const uint32_t steps = (rest + 15u) / 16u;  // MMAs of 16 rows that hold any
+                            const uint32_t words = (steps * 16u - rest) * 8u;  // 16-byte words behind the end, per box
+                            for (uint32_t i = lane; i < words * 4u; i += 32u) {
+                                const uint32_t box = i / words, w = i - box * words;
+                                // four boxes of 8 KB, one behind the other: two of P, two of Q
+                                *reinterpret_cast<uint4 *>(base_ptr + stage * T::kStageBytes + box * 8192u + rest * 128u + w * 16u) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (CG == 2) mbar_arrive_cluster(map_to_cta(ready_bar + 8u * stage, 0));
+                                if (cta_rank == 0) {
+                                    if (CG == 2) {
+                                        // both CTAs have cleared their parts, and the stage's own barrier has passed its phase
+                                        if (!mbar_wait(ready_bar + 8u * stage, parity, abort_flag) ||
+                                            !mbar_wait(full_bar + 8u * stage, phase, abort_flag)) {
+                                            ok = false;
+                                        } else {
+                                            mbar_try_wait_cluster(ready_bar + 8u * stage, parity);
+                                        }
+                                    }
+                                    if (ok) {
+                                        tcgen05_fence_after_sync();
+                                        const uint64_t dp = umma_smem_desc_sw128_mn(slot, 8192u);
+                                        const uint64_t dq = umma_smem_desc_sw128_mn(slot + T::kPBytes, 8192u);
+                                        for (uint32_t k = 0; k < steps; ++k) {
+                                            umma_f16<CG>(d_tmem, dp + 128u * k, dq + 128u * k, idesc, (blocks > 1u || k > 0) ? 1u : 0u);
+                                        }
+                                        if (CG == 1) umma_commit(empty_bar + 8u * stage); else umma_commit_pair(empty_bar + 8u * stage, 0x3);
+                                    }
+                                }
+                            }
+                        } else {
+                            ok = false;
+                        }
+                        ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                        tail_phase ^= 1u << stage;
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+                if (cta_rank == 0 && lane == 0 && ok) {
+                    if (CG == 1) umma_commit(tfull_bar + 8u * acc); else umma_commit_pair(tfull_bar + 8u * acc, 0x3);
+                }
+                if (!WEIGHT) ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                ++it;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------ epilogue
+        const uint32_t q = warp & 3u;  // tensor-memory lane quadrant this warp may read
+        uint32_t it = 0, store_buf = 0;
+        for (uint32_t t = worker; t < tiles; t += workers) {
+            GroupedTile tile;
+            if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
+            const bool summed = !WEIGHT || tile.valid != 0;  // a group without rows: a gradient of zeros, no accumulator
+            const uint32_t acc = it & 1u;
+            if (summed) {
+                uint32_t ready = 1;
+                if (lane == 0) ready = mbar_wait(tfull_bar + 8u * acc, (it >> 1) & 1u, abort_flag) ? 1u : 0u;
+                ready = __shfl_sync(0xffffffffu, ready, 0);
+                if (!ready) break;
+                tcgen05_fence_after_sync();
+            }
+            const uint32_t taddr = tmem_base + ((q * 32u) << 16) + acc * QT;
+            const uint32_t p_warp = tile.p0 + cta_rank * 128u + q * 32u;  // first index on P of this warp's lanes
+            if (!WEIGHT) {
+                const uint32_t col = p_warp + lane;
+                float bias = 0.f;
+                if (FORM == kFormForward && p.bias && col < p.p_dim) {
+                    const size_t at = static_cast<size_t>(tile.group) * p.p_dim + col;
+                    bias = p.in_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[at])
+                                     : __half2float(static_cast<const __half *>(p.bias)[at]);
+                }
+                if (p_warp < p.p_dim) {
+#pragma unroll 1
+                    for (uint32_t c = 0; c * 32u < tile.valid; ++c) {
+                        uint32_t r[32];
+                        tmem_ld_32x32b_x32(taddr + c * 32u, r);
+                        tmem_ld_wait();
+                        if (FORM == kFormForward) {
+                            if (p.bias) {
+#pragma unroll
+                                for (uint32_t j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + bias);
+                            }
+                            if (p.pre) store_transposed32(p.pre, p.out_type, tile.q0 + c * 32u, tile.valid - c * 32u, col, p.p_dim, r, lane);
+                            act_apply<32>(r, p.act);
+                        }
+                        store_transposed32(p.out, p.out_type, tile.q0 + c * 32u, tile.valid - c * 32u, col, p.p_dim, r, lane);
+                    }
+                }
+            } else if (p_warp < p.p_dim && (summed || !p.accumulate)) {
+                // rows of the result: through swizzled staging (32 rows of 128 bytes) and TMA, which clips what lies
+                // past N and K; with `accumulate` the copy adds to what is there
+                const bool f32 = p.out_type == 2u;
+                uint8_t *my_ptr = staging_ptr + q * 8192u;
+                const uint32_t my_staging = staging + q * 8192u;
+                const uint32_t width = f32 ? 32u : 64u;  // columns of 128 bytes
+                const uint32_t cols = min(static_cast<uint32_t>(QT), p.q_dim - tile.q0);
+#pragma unroll 1
+                for (uint32_t c0 = 0; c0 < cols; c0 += width) {
+                    uint8_t *row_ptr = my_ptr + (store_buf & 1u) * 4096u + lane * 128u;
+                    if (lane == 0) tma_store_wait_read<1>();  // the store issued two chunks ago has read this buffer
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t part = 0; part * 32u < width; ++part) {
+                        uint32_t r[32];
+                        if (summed) {
+                            tmem_ld_32x32b_x32(taddr + c0 + part * 32u, r);
+                            tmem_ld_wait();
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < 32; ++j) r[j] = 0u;
+                        }
+                        if (f32) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 8; ++j) {
+                                *reinterpret_cast<uint4 *>(row_ptr + ((j ^ (lane & 7u)) << 4)) =
+                                    make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                uint4 v;
+                                v.x = pack2_typed(r[8 * j + 0], r[8 * j + 1], p.out_type);
+                                v.y = pack2_typed(r[8 * j + 2], r[8 * j + 3], p.out_type);
+                                v.z = pack2_typed(r[8 * j + 4], r[8 * j + 5], p.out_type);
+                                v.w = pack2_typed(r[8 * j + 6], r[8 * j + 7], p.out_type);
+                                *reinterpret_cast<uint4 *>(row_ptr + (((part * 4u + j) ^ (lane & 7u)) << 4)) = v;
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const uint32_t src = my_staging + (store_buf & 1u) * 4096u;
+                        const int32_t x = static_cast<int32_t>(tile.q0 + c0), y = static_cast<int32_t>(p_warp);
+                        const int32_t z = static_cast<int32_t>(tile.group);
+                        if (p.accumulate) tma_reduce_add_3d(&p.tm_out, src, x, y, z); else tma_store_3d(&p.tm_out, src, x, y, z);
+                        tma_store_commit();
+                    }
+                    ++store_buf;
+                }
+            }
+            if (summed) {
+                tcgen05_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 1) mbar_arrive(tempty_bar + 8u * acc); else mbar_arrive_cluster(map_to_cta(tempty_bar + 8u * acc, 0));
+                }
+                ++it;
+            }
+        }
+        if (WEIGHT && lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+    }
+
+    // ---------------------------------------------------------------------- teardown
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        // give copies still in flight time to land before shared memory is released
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) {
+        }
+        if (threadIdx.x == 0) atomicExch(p.error_word, 1u);
+        __syncthreads();
+    }
+    if (CG == 2) cluster_sync_all();
+    if (warp == 1) {
+        tcgen05_fence_after_sync();
+        tmem_dealloc<CG>(tmem_base, T::kTmemCols);
+    }
+}
+
+}  // namespace b200

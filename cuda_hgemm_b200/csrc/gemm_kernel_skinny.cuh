@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
         if (lane == 0 && cta_rank == 0) {
-            constexpr uint32_t idesc = umma_idesc_f16_f32(128 * CG, MT);
+            const uint32_t idesc = umma_idesc_f16_f32(128 * CG, MT) | (EPI && p.epi.in_bf16 ? kUmmaIdescBf16 : 0u);
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t kb = kb0; kb < kb1; kb += KPS) {

@@ -1,0 +1,385 @@
+// Host side of the feed-forward products (include/b200_hgemm.h): argument checks, the choice of tile and the
+// launches of the grouped kernel in its three forms and of the pass over an output's gradient.
+#include <string.h>
+
+#include "../../include/b200_hgemm.h"
+#include "gemm_kernel_grouped.cuh"
+#include "lib_state.h"
+#include "slope_kernel.cuh"
+
+#include <initializer_list>
+
+namespace b200 {
+
+static bool known_act(int32_t act) {
+    return act >= B200_ACT_NONE && act <= B200_ACT_SILU;
+}
+
+// Types a caller may name: 16-bit inputs, and outputs of that type or FP32.
+static bool known_types(int32_t in_type, int32_t out_type) {
+    return (in_type == B200_C_F16 || in_type == B200_C_BF16) && (out_type == in_type || out_type == B200_C_F32);
+}
+
+static bool misaligned(std::initializer_list<const void *> ptrs) {
+    uintptr_t bits = 0;
+    for (const void *p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+    return (bits & 15u) != 0;
+}
+
+// Kernel attributes of one launch: programmatic dependent launch, and the pair where there is one.
+static int launch_attributes(cudaLaunchAttribute *attrs, int cg) {
+    int n = 0;
+    if (pdl_enabled()) {
+        attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    if (cg == 2) {
+        attrs[n].id = cudaLaunchAttributeClusterDimension;
+        attrs[n].val.clusterDim.x = 2;
+        attrs[n].val.clusterDim.y = 1;
+        attrs[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    return n;
+}
+
+// `most_tiles`: an upper bound of the tiles there can be; the grid is persistent and never larger than what
+// is resident at once.
+template <int FORM, int CG, int QT, int STAGES, int KPS>
+static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uint64_t most_tiles, cudaStream_t stream) {
+    using T = GroupedTraits<FORM, CG, QT, STAGES, KPS>;
+    auto kern = hgemm_grouped_kernel<FORM, CG, QT, STAGES, KPS>;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attrs[2];
+    cfg.blockDim = dim3(kGroupedThreads, 1, 1);
+    cfg.dynamicSmemBytes = T::kSmemBytes;
+    cfg.stream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = launch_attributes(attrs, CG);
+    uint32_t resident = static_cast<uint32_t>(st.sm_count);
+    {
+        std::lock_guard<std::mutex> lock(st.mu);
+        if (!st.attr_set[slot]) {
+            if (!cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmemBytes), "cudaFuncSetAttribute")) {
+                return B200_HGEMM_ERR_CUDA;
+            }
+            st.attr_set[slot] = true;
+        }
+        if (CG == 2) {
+            if (st.max_clusters[slot] == 0) {
+                int n = 0;
+                cfg.gridDim = dim3(2u * (st.sm_count / 2), 1, 1);
+                if (!cuda_ok(cudaOccupancyMaxActiveClusters(&n, kern, &cfg), "cudaOccupancyMaxActiveClusters") || n < 1) {
+                    return B200_HGEMM_ERR_CUDA;
+                }
+                st.max_clusters[slot] = n;
+            }
+            resident = static_cast<uint32_t>(st.max_clusters[slot]);
+        }
+    }
+    const uint32_t workers = most_tiles < resident ? static_cast<uint32_t>(most_tiles) : resident;
+    cfg.gridDim = dim3(workers * CG, 1, 1);
+    if (!cuda_ok(cudaLaunchKernelEx(&cfg, kern, p), "cudaLaunchKernelEx")) return B200_HGEMM_ERR_CUDA;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return B200_HGEMM_OK;
+}
+
+// Forward and input form. X: the rows' operand [rows x k_dim]; W: groups matrices [w_rows x w_cols], stride_w apart.
+template <int FORM>
+static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, size_t p_dim, size_t k_dim, size_t w_rows,
+                    size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, cudaStream_t stream) {
+    constexpr int kSlots = FORM == kFormForward ? 96 : 100;
+    p.error_word = st.error_word;
+    p.rows = static_cast<uint32_t>(rows);
+    p.groups = static_cast<uint32_t>(groups);
+    p.p_dim = static_cast<uint32_t>(p_dim);
+    // Tile: pairs on 256 x 256 once they fill the GPU; single CTAs on 128 columns of weights and up to 128 rows
+    // below that, with blocks of rows halved until every SM has a tile; and where the groups hold no more than 32 rows
+    // on average, a ring of weights with little room for rows (decode: bound by reading the weights once).
+    const uint64_t average = (rows + groups - 1) / groups;
+    const uint64_t sms = static_cast<uint64_t>(st.sm_count);
+    auto most_tiles = [&](uint64_t width, uint64_t q_max) {
+        const uint64_t blocks = rows / q_max + (groups < rows ? groups : rows);
+        return blocks * ceil_div_u32(p_dim, width);
+    };
+    auto few_tiles = [&](uint64_t width, uint64_t q_max) {
+        const uint64_t blocks = (average + q_max - 1) / q_max * (groups < rows ? groups : rows);
+        return blocks * ceil_div_u32(p_dim, width);
+    };
+    int cg = 1, kps = 2;
+    uint32_t q_cap = 32;
+    p.q_max = 32;
+    if (average > 32) {
+        if (few_tiles(256, 256) >= sms / 2) {
+            cg = 2;
+            kps = 1;
+            q_cap = 256;
+            p.q_max = 256;
+        } else {
+            q_cap = 128;
+            p.q_max = 128;
+            while (p.q_max > 32 && few_tiles(128, p.q_max) < sms) p.q_max /= 2;
+        }
+    }
+    p.p_blocks = ceil_div_u32(p_dim, 128u * cg);
+    p.p_div = make_fast_div(p.p_blocks);
+    p.k_blocks = ceil_div_u32(k_dim, 64u * kps);
+    const uint64_t tiles = most_tiles(128u * cg, p.q_max);
+    if (tiles > 0x7fffffffull) return B200_HGEMM_ERR_TOO_LARGE;
+    int rc;
+    const uint32_t box_rows = FORM == kFormForward ? 128u : 64u;
+    if ((rc = get_tensor_map(st, W, w_rows, w_cols, box_rows, 64, &p.tm_p, true, groups, stride_w)) != B200_HGEMM_OK) return rc;
+    for (uint32_t i = 0; i < 4; ++i) {
+        if ((rc = get_tensor_map(st, X, rows, k_dim, 128u >> i, 64, &p.tm_q[i])) != B200_HGEMM_OK) return rc;
+    }
+    if (cg == 2) return launch_grouped<FORM, 2, 256, 6, 1>(st, kSlots, p, tiles, stream);
+    if (q_cap == 128) return launch_grouped<FORM, 1, 128, 3, 2>(st, kSlots + 1, p, tiles, stream);
+    return launch_grouped<FORM, 1, 32, 5, 2>(st, kSlots + 2, p, tiles, stream);
+}
+
+// Weight form: dB_g = dZ_g^T A_g.
+static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, const int32_t *offsets, size_t M, size_t N, size_t K,
+                      size_t G, const b200_linear_grads &g, cudaStream_t stream) {
+    GroupedParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = dB;
+    p.offsets = offsets;
+    p.error_word = st.error_word;
+    p.rows = static_cast<uint32_t>(M);
+    p.groups = static_cast<uint32_t>(G);
+    p.p_dim = static_cast<uint32_t>(N);
+    p.q_dim = static_cast<uint32_t>(K);
+    p.in_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
+    p.out_type = static_cast<uint32_t>(g.db_type);
+    p.accumulate = g.accumulate ? 1u : 0u;
+    const uint64_t pair_tiles = static_cast<uint64_t>(G) * ceil_div_u32(N, 256) * ceil_div_u32(K, 256);
+    const int cg = pair_tiles >= static_cast<uint64_t>(st.sm_count) / 2 ? 2 : 1;
+    p.p_blocks = ceil_div_u32(N, 128u * cg);
+    p.q_blocks = ceil_div_u32(K, 128u * cg);
+    p.p_div = make_fast_div(p.p_blocks);
+    const uint64_t tiles = static_cast<uint64_t>(G) * p.p_blocks * p.q_blocks;
+    if (tiles > 0x7fffffffull) return B200_HGEMM_ERR_TOO_LARGE;
+    int rc;
+    if ((rc = get_tensor_map(st, dZ, M, N, 64, 64, &p.tm_p)) != B200_HGEMM_OK) return rc;
+    if ((rc = get_tensor_map(st, A, M, K, 64, 64, &p.tm_q[0])) != B200_HGEMM_OK) return rc;
+    const bool f32 = g.db_type == B200_C_F32;
+    if ((rc = get_tensor_map(st, dB, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
+    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 104, p, tiles, stream);
+    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 105, p, tiles, stream);
+}
+
+// ---- the pass over dC -----------------------------------------------------------------------
+// Slices a group's rows are cut into: about 128 rows each where the groups are even, four times as many where there
+// are several (one may hold much more than its share), and enough blocks to fill the GPU when there are few rows.
+static uint32_t slope_slices(size_t M, size_t N, size_t G) {
+    const uint64_t spread = G < 4 ? G : 4;
+    uint64_t slices = (M * spread + 128 * G - 1) / (128 * G);
+    const uint64_t strips = ceil_div_u32(N, kSlopeColumns);
+    const uint64_t fill = 296 / (strips * G) + 1, most = (M + 15) / 16;
+    if (slices < fill) slices = fill;
+    if (slices > most) slices = most;
+    if (slices > 4096) slices = 4096;
+    return slices < 1 ? 1u : static_cast<uint32_t>(slices);
+}
+
+// Whether the products read a dZ other than the caller's dC.
+static bool needs_dz(const b200_linear_grads &g) {
+    return g.act != B200_ACT_NONE || g.c_type != g.in_type;
+}
+
+static size_t align256(size_t v) {
+    return (v + 255) / 256 * 256;
+}
+
+static size_t dz_bytes(size_t M, size_t N, const b200_linear_grads &g) {
+    return (!g.dZ && needs_dz(g) && (g.dA || g.dB)) ? align256(M * N * 2) : 0;
+}
+
+static size_t sums_bytes(size_t M, size_t N, size_t G, const b200_linear_grads &g) {
+    const uint32_t slices = slope_slices(M, N, G);
+    return g.dbias && slices > 1 ? align256(static_cast<size_t>(slices) * G * N * sizeof(float)) : 0;
+}
+
+static int launch_slope(const SlopeParams &p, uint32_t act, dim3 grid, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attrs[2];
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kSlopeThreads, 1, 1);
+    cfg.stream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = launch_attributes(attrs, 1);
+    cudaError_t e;
+    switch (act) {
+        case kActRelu: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActRelu>, p); break;
+        case kActGelu: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActGelu>, p); break;
+        case kActGeluTanh: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActGeluTanh>, p); break;
+        case kActSilu: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActSilu>, p); break;
+        default: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActNone>, p); break;
+    }
+    if (!cuda_ok(e, "cudaLaunchKernelEx")) return B200_HGEMM_ERR_CUDA;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return B200_HGEMM_OK;
+}
+
+static int run_slope(const b200_linear_grads &g, void *dz, float *sums, const int32_t *offsets, size_t M, size_t N, size_t G,
+                     cudaStream_t stream) {
+    SlopeParams p;
+    memset(&p, 0, sizeof(p));
+    p.dc = g.dC;
+    p.pre = g.pre;
+    p.dz = dz;
+    p.offsets = offsets;
+    p.rows = static_cast<uint32_t>(M);
+    p.n = static_cast<uint32_t>(N);
+    p.groups = static_cast<uint32_t>(G);
+    p.slices = slope_slices(M, N, G);
+    p.c_type = static_cast<uint32_t>(g.c_type);
+    p.dz_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
+    const bool one = p.slices == 1;
+    p.sums = g.dbias ? (one ? g.dbias : sums) : nullptr;
+    p.accumulate = one && g.accumulate ? 1u : 0u;
+    const dim3 grid(ceil_div_u32(N, kSlopeColumns), p.slices, static_cast<unsigned>(G));
+    int rc = launch_slope(p, static_cast<uint32_t>(g.act), grid, stream);
+    if (rc != B200_HGEMM_OK || !g.dbias || one) return rc;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attrs[2];
+    const size_t count = G * N;
+    cfg.gridDim = dim3(ceil_div_u32(count, 256), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = launch_attributes(attrs, 1);
+    if (!cuda_ok(cudaLaunchKernelEx(&cfg, bias_sum_kernel, static_cast<const float *>(sums), g.dbias, count, p.slices,
+                                    g.accumulate ? 1u : 0u),
+                 "cudaLaunchKernelEx")) {
+        return B200_HGEMM_ERR_CUDA;
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return B200_HGEMM_OK;
+}
+
+static int check_sizes(size_t M, size_t N, size_t K) {
+    if (N == 0 || K == 0) return B200_HGEMM_ERR_INVALID_ARG;
+    if (M > 0x7fffff00ull || N > 0x7fffff00ull || K > 0x7fffff00ull) return B200_HGEMM_ERR_UNSUPPORTED;
+    return B200_HGEMM_OK;
+}
+
+static int check_groups(const int32_t *offsets, size_t N, size_t K, size_t G, size_t stride_b) {
+    if (!offsets || G == 0) return B200_HGEMM_ERR_INVALID_ARG;
+    if (G > kGroupedMaxGroups) return B200_HGEMM_ERR_TOO_LARGE;
+    if ((reinterpret_cast<uintptr_t>(offsets) & 3u) != 0 || stride_b % 8 != 0) return B200_HGEMM_ERR_MISALIGNED;
+    if (G > 1 && stride_b < N * K) return B200_HGEMM_ERR_INVALID_ARG;
+    return B200_HGEMM_OK;
+}
+
+static int grouped_forward(const void *A, const void *B, void *C, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
+                           size_t stride_b, const b200_linear_args *args, cudaStream_t stream) {
+    if (!args || !B || (M > 0 && (!A || !C))) return B200_HGEMM_ERR_INVALID_ARG;
+    int rc = check_sizes(M, N, K);
+    if (rc != B200_HGEMM_OK) return rc;
+    if ((rc = check_groups(offsets, N, K, G, stride_b)) != B200_HGEMM_OK) return rc;
+    if (!known_act(args->act) || !known_types(args->in_type, args->c_type)) return B200_HGEMM_ERR_INVALID_ARG;
+    if (args->residual || K % 8 != 0) return B200_HGEMM_ERR_UNSUPPORTED;
+    if (misaligned({A, B, C, args->bias, args->pre})) return B200_HGEMM_ERR_MISALIGNED;
+    if (M == 0) return B200_HGEMM_OK;
+    DeviceState *st = nullptr;
+    if ((rc = current_state(&st)) != B200_HGEMM_OK) return rc;
+    if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
+    GroupedParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = C;
+    p.pre = args->pre;
+    p.bias = args->bias;
+    p.offsets = offsets;
+    p.in_bf16 = args->in_type == B200_C_BF16 ? 1u : 0u;
+    p.out_type = static_cast<uint32_t>(args->c_type);
+    p.act = static_cast<uint32_t>(args->act);
+    return run_rows<kFormForward>(*st, A, B, M, N, K, N, K, G, G > 1 ? stride_b : N * K, p, stream);
+}
+
+// Both backward entry points; `offsets` is null for the dense one.
+static int backward(const void *A, const void *B, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G, size_t stride_b,
+                    const b200_linear_grads *grads, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    if (!grads) return B200_HGEMM_ERR_INVALID_ARG;
+    const b200_linear_grads &g = *grads;
+    int rc = check_sizes(M, N, K);
+    if (rc != B200_HGEMM_OK) return rc;
+    if (!known_act(g.act) || !known_types(g.in_type, g.c_type)) return B200_HGEMM_ERR_INVALID_ARG;
+    if (g.db_type != g.in_type && g.db_type != B200_C_F32) return B200_HGEMM_ERR_INVALID_ARG;
+    if (M > 0 && (!g.dC || (g.act != B200_ACT_NONE && !g.pre))) return B200_HGEMM_ERR_INVALID_ARG;
+    if (M > 0 && ((g.dA && !B) || (g.dB && !A))) return B200_HGEMM_ERR_INVALID_ARG;
+    if (M > 0 && !g.dA && !g.dB && !g.dbias && !g.dZ) return B200_HGEMM_ERR_INVALID_ARG;
+    if (N % 8 != 0 || K % 8 != 0) return B200_HGEMM_ERR_UNSUPPORTED;
+    if (g.accumulate && g.dB && g.db_type != B200_C_F32) return B200_HGEMM_ERR_UNSUPPORTED;
+    if (misaligned({A, B, g.dC, g.pre, g.dZ, g.dA, g.dB, g.dbias})) return B200_HGEMM_ERR_MISALIGNED;
+    const size_t need_dz = dz_bytes(M, N, g), need_sums = sums_bytes(M, N, G, g);
+    if (need_dz + need_sums > 0) {
+        if (!workspace || workspace_bytes < need_dz + need_sums) return B200_HGEMM_ERR_WORKSPACE;
+        if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200_HGEMM_ERR_MISALIGNED;
+    }
+    DeviceState *st = nullptr;
+    if ((rc = current_state(&st)) != B200_HGEMM_OK) return rc;
+    if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
+    if (M == 0) {
+        // nothing was multiplied: the gradients of the weights are zeros
+        if (g.accumulate) return B200_HGEMM_OK;
+        const size_t db_bytes = G * N * K * (g.db_type == B200_C_F32 ? 4 : 2);
+        if (g.dB && !cuda_ok(cudaMemsetAsync(g.dB, 0, db_bytes, stream), "cudaMemsetAsync")) return B200_HGEMM_ERR_CUDA;
+        if (g.dbias && !cuda_ok(cudaMemsetAsync(g.dbias, 0, G * N * sizeof(float), stream), "cudaMemsetAsync")) return B200_HGEMM_ERR_CUDA;
+        return B200_HGEMM_OK;
+    }
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    void *dz = g.dZ ? g.dZ : (need_dz ? ws : nullptr);
+    float *sums = reinterpret_cast<float *>(ws + need_dz);
+    if (dz || g.dbias) {
+        if ((rc = run_slope(g, dz, sums, offsets, M, N, G, stream)) != B200_HGEMM_OK) return rc;
+    }
+    const void *dz_read = needs_dz(g) ? dz : g.dC;
+    if (g.dA) {
+        GroupedParams p;
+        memset(&p, 0, sizeof(p));
+        p.out = g.dA;
+        p.offsets = offsets;
+        p.in_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
+        p.out_type = static_cast<uint32_t>(g.in_type);
+        rc = run_rows<kFormInput>(*st, dz_read, B, M, K, N, N, K, G, G > 1 ? stride_b : N * K, p, stream);
+        if (rc != B200_HGEMM_OK) return rc;
+    }
+    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, stream);
+    return B200_HGEMM_OK;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_hgemm_grouped(const void *A, const void *B, void *C, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
+                       size_t stride_b, const b200_linear_args *args, b200_stream_t stream) {
+    return grouped_forward(A, B, C, offsets, M, N, K, G, stride_b, args, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b200_hgemm_grouped_backward(const void *A, const void *B, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
+                                size_t stride_b, const b200_linear_grads *grads, void *workspace, size_t workspace_bytes,
+                                b200_stream_t stream) {
+    const int rc = N == 0 || K == 0 ? B200_HGEMM_ERR_INVALID_ARG : check_groups(offsets, N, K, G, stride_b);
+    if (rc != B200_HGEMM_OK) return rc;
+    return backward(A, B, offsets, M, N, K, G, stride_b, grads, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b200_hgemm_linear_backward(const void *A, const void *B, size_t M, size_t N, size_t K, const b200_linear_grads *grads,
+                               void *workspace, size_t workspace_bytes, b200_stream_t stream) {
+    return backward(A, B, nullptr, M, N, K, 1, N * K, grads, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t b200_hgemm_backward_workspace_bytes(size_t M, size_t N, size_t K, size_t G, const b200_linear_grads *grads) {
+    if (!grads || N == 0 || K == 0 || G == 0) return 0;
+    return dz_bytes(M, N, *grads) + sums_bytes(M, N, G, *grads);
+}
+
+}  // extern "C"

@@ -23,68 +23,16 @@
 #include "gemm_kernel.cuh"
 #include "gemm_kernel_big.cuh"
 #include "gemm_kernel_skinny.cuh"
+#include "lib_state.h"
 
 namespace b200 {
 
 // ------------------------------------------------------------------------------------------
 // per-device state
 // ------------------------------------------------------------------------------------------
-constexpr int kMaxDevices = 64;
 constexpr size_t kMaxOwnedWorkspace = size_t(1) << 30;  // the library never grows its own workspace past 1 GiB
 constexpr size_t kCounterBytes = 64 * 1024;             // reserved header at the front of the workspace (no kernel uses it now)
 constexpr uint32_t kMaxCountedTiles = kCounterBytes / 4;  // most tiles the allocation-free stream-k entry point accepts
-
-struct TensorMapKey {
-    const void *ptr;
-    uint64_t rows, cols;
-    uint32_t box_rows, box_cols;
-    bool swizzle;
-    uint64_t batch, batch_stride;  // stacks of matrices: how many, and elements from one to the next (1, 0: a single matrix)
-    bool operator==(const TensorMapKey &o) const {
-        return ptr == o.ptr && rows == o.rows && cols == o.cols && box_rows == o.box_rows && box_cols == o.box_cols &&
-               swizzle == o.swizzle && batch == o.batch && batch_stride == o.batch_stride;
-    }
-};
-
-struct TensorMapSlot {
-    bool used = false;
-    uint64_t last_use = 0;
-    TensorMapKey key{};
-    CUtensorMap map{};
-};
-constexpr size_t kTensorMapWays = 4;
-
-struct DeviceState {
-    std::mutex mu;
-    bool probed = false;       // attributes known and the error word allocated
-    bool attrs_known = false;  // sm100 / sm_count filled in (no allocation needed for that)
-    bool sm100 = false;
-    int sm_count = 0;
-    uint32_t *error_word = nullptr;
-    // stream-k workspace [64 KiB header | FP32 partial slots]: either one the caller handed over
-    // (ws), or one per stream that the library allocates and grows itself, so that GEMMs running
-    // on different streams at the same time never share partial-tile slots
-    void *ws = nullptr;
-    size_t ws_bytes = 0;
-    struct StreamWorkspace {
-        cudaStream_t stream;
-        void *ptr;
-        size_t bytes;
-        uint64_t last_use;
-    };
-    std::vector<StreamWorkspace> owned_ws;
-    uint64_t ws_clock = 0;
-    // staging buffers of the host-pointer entry point
-    void *host_a = nullptr, *host_b = nullptr, *host_c = nullptr;
-    size_t host_a_bytes = 0, host_b_bytes = 0, host_c_bytes = 0;
-    cudaStream_t host_stream[3] = {nullptr, nullptr, nullptr};  // upload, GEMMs, download
-    cudaEvent_t host_event[2] = {nullptr, nullptr};
-    bool attr_set[96] = {};
-    int max_clusters[96] = {};
-    int ck_clusters[16][9] = {};  // short-A kernels that sum inside clusters: clusters of each size the device holds at once (-1: none)  // CTA pairs the device can keep resident at once, per pair kernel
-    TensorMapSlot tm_cache[64 * kTensorMapWays];
-    uint64_t tm_clock = 0;
-};
 
 static DeviceState g_dev[kMaxDevices];
 #ifdef B200_TIMELINE
@@ -92,11 +40,11 @@ static DeviceState g_dev[kMaxDevices];
 static unsigned long long *g_timeline = nullptr;
 extern "C" void b200_debug_set_timeline(unsigned long long *buf) { g_timeline = buf; }
 #endif
-static std::atomic<uint64_t> g_launches{0};
+std::atomic<uint64_t> g_launches{0};
 
 // With B200_HGEMM_DEBUG set in the environment, every failing CUDA call is named on stderr
 // (the C ABI itself only returns B200_HGEMM_ERR_CUDA).
-static bool cuda_ok(cudaError_t e, const char *what) {
+bool cuda_ok(cudaError_t e, const char *what) {
     if (e == cudaSuccess) return true;
     static const bool verbose = (getenv("B200_HGEMM_DEBUG") != nullptr);
     if (verbose) fprintf(stderr, "[b200_hgemm] %s failed: %s\n", what, cudaGetErrorString(e));
@@ -135,7 +83,7 @@ static int probe_attributes_locked(DeviceState &st, int dev) {
     return B200_HGEMM_OK;
 }
 
-static int current_state(DeviceState **out) {
+int current_state(DeviceState **out) {
     int dev = 0;
     if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return B200_HGEMM_ERR_CUDA;
     if (dev < 0 || dev >= kMaxDevices) return B200_HGEMM_ERR_CUDA;
@@ -163,16 +111,16 @@ static int current_state(DeviceState **out) {
     return B200_HGEMM_OK;
 }
 
-// A 2-D FP16 tensor of `rows` x `cols` (cols contiguous) viewed through boxes of
+// A 2-D tensor (16-bit elements, or FP32 with elem_bytes = 4) of `rows` x `cols` (cols contiguous) viewed through boxes of
 // box_rows x box_cols, with the 128-byte swizzle (box_cols = 64) or, for plain row-major staging
 // tiles, without. Out-of-range elements read as zero and are dropped on store. The cache is 4-way
 // set-associative (64 sets): a handful of operands in rotation never evict each other.
-static int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows,
-                          uint32_t box_cols, CUtensorMap *out, bool swizzle = true, uint64_t batch = 1, uint64_t batch_stride = 0) {
-    TensorMapKey key{ptr, rows, cols, box_rows, box_cols, swizzle, batch, batch_stride};
+int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
+                   CUtensorMap *out, bool swizzle, uint64_t batch, uint64_t batch_stride, uint32_t elem_bytes) {
+    TensorMapKey key{ptr, rows, cols, box_rows, box_cols, swizzle, batch, batch_stride, elem_bytes};
     size_t h = (reinterpret_cast<uintptr_t>(ptr) >> 8) * 0x9E3779B97F4A7C15ull;
     h ^= rows * 0xC2B2AE3D27D4EB4Full + cols * 0x165667B19E3779F9ull + box_rows * 131u + box_cols + (swizzle ? 0u : 77u) +
-         batch * 0x9E3779B1ull + batch_stride * 0x85EBCA77ull;
+         batch * 0x9E3779B1ull + batch_stride * 0x85EBCA77ull + elem_bytes;
     const size_t set = ((h >> 20) & 63u) * kTensorMapWays;
     std::lock_guard<std::mutex> lock(st.mu);
     TensorMapSlot *slot = nullptr;
@@ -191,10 +139,10 @@ static int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint6
     // a stack of matrices is a third dimension; a stack of one with stride 0 stays two-dimensional
     const bool stacked = batch > 1 || batch_stride != 0;
     cuuint64_t dims[3] = {cols, rows, batch};
-    cuuint64_t strides[2] = {cols * sizeof(__half), (batch_stride ? batch_stride : rows * cols) * sizeof(__half)};
+    cuuint64_t strides[2] = {cols * elem_bytes, (batch_stride ? batch_stride : rows * cols) * elem_bytes};
     cuuint32_t box[3] = {box_cols, box_rows, 1};
     cuuint32_t elem_strides[3] = {1, 1, 1};
-    CUresult r = enc(&slot->map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, stacked ? 3 : 2, const_cast<void *>(ptr), dims, strides, box,
+    CUresult r = enc(&slot->map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, stacked ? 3 : 2, const_cast<void *>(ptr), dims, strides, box,
                      elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
@@ -297,10 +245,6 @@ static McLaunchFn mc_launch_fn(int bn = 256) {
 // ------------------------------------------------------------------------------------------
 // plans
 // ------------------------------------------------------------------------------------------
-static inline uint32_t ceil_div_u32(uint64_t a, uint64_t b) {
-    return static_cast<uint32_t>((a + b - 1) / b);
-}
-
 // STREAMK and HYBRID run the same kernel; HYBRID walks the full waves of tiles whole first. HYBRID_PAIR is
 // HYBRID on CTA pairs (256-row tiles).
 static bool plan_cuts_k(const b200_hgemm_plan &pl) {
@@ -649,7 +593,7 @@ static void select_plan(const DeviceState &st, size_t M, size_t N, size_t K, b20
 // ------------------------------------------------------------------------------------------
 // Programmatic dependent launch is on unless B200_HGEMM_NO_PDL is set in the environment (for
 // A/B measurements; without the launch attribute the kernels' griddepcontrol instructions do nothing).
-static bool pdl_enabled() {
+bool pdl_enabled() {
     static const bool on = (getenv("B200_HGEMM_NO_PDL") == nullptr);
     return on;
 }
@@ -901,16 +845,29 @@ static int run_simt(const void *A, const void *B, void *C, size_t M, size_t N, s
     return B200_HGEMM_OK;
 }
 
+// What either entry point with an epilogue asks of the kernels: b200_hgemm_fused's part, and what a linear layer
+// adds to it (zeros otherwise).
+struct LibEpilogue : b200_hgemm_epilogue {
+    uint32_t act = kActNone;
+    uint32_t in_bf16 = 0;
+    void *pre = nullptr;
+};
+
 // The fused epilogue a caller asked for, checked and in the kernels' terms.
-static int epilogue_args(const b200_hgemm_epilogue &epi, EpilogueArgs *out) {
+static int epilogue_args(const LibEpilogue &epi, EpilogueArgs *out) {
     if (epi.c_type != B200_C_F16 && epi.c_type != B200_C_BF16 && epi.c_type != B200_C_F32) return B200_HGEMM_ERR_INVALID_ARG;
     if (epi.beta != 0.f && !epi.c_in) return B200_HGEMM_ERR_INVALID_ARG;
-    if ((reinterpret_cast<uintptr_t>(epi.bias) | reinterpret_cast<uintptr_t>(epi.c_in)) & 15u) return B200_HGEMM_ERR_MISALIGNED;
+    if ((reinterpret_cast<uintptr_t>(epi.bias) | reinterpret_cast<uintptr_t>(epi.c_in) | reinterpret_cast<uintptr_t>(epi.pre)) & 15u) {
+        return B200_HGEMM_ERR_MISALIGNED;
+    }
     out->alpha = epi.alpha;
     out->beta = epi.beta;
     out->bias = static_cast<const __half *>(epi.bias);
     out->c_in = epi.c_in;
     out->c_type = static_cast<uint32_t>(epi.c_type);
+    out->act = epi.act;
+    out->pre = epi.pre;
+    out->in_bf16 = epi.in_bf16;
     return B200_HGEMM_OK;
 }
 
@@ -1093,7 +1050,7 @@ static int launch_skinny_kernel(DeviceState &st, int attr_slot, const SkinnyPara
 
 static int run_skinny(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K,
                       const b200_hgemm_plan &pl, cudaStream_t stream, void *ws_override, size_t ws_override_bytes,
-                      uint32_t *error_word, const b200_hgemm_epilogue *epi) {
+                      uint32_t *error_word, const LibEpilogue *epi) {
     if (M > static_cast<size_t>(pl.bn)) return B200_HGEMM_ERR_UNSUPPORTED;
     SkinnyParams p;
     memset(&p, 0, sizeof(p));
@@ -1230,7 +1187,7 @@ static int launch_big_with_tail(DeviceState &st, const GemmParams &p, uint32_t g
 
 static int run_plan(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K,
                     const b200_hgemm_plan &pl, cudaStream_t stream, void *ws_override, size_t ws_override_bytes,
-                    uint32_t *error_word_override = nullptr, const b200_hgemm_epilogue *epi = nullptr) {
+                    uint32_t *error_word_override = nullptr, const LibEpilogue *epi = nullptr) {
     int rc = validate_plan(pl, N, K);
     if (rc != B200_HGEMM_OK) return rc;
     if (pl.variant == B200_VARIANT_SIMT) return run_simt(A, B, C, M, N, K, stream);
@@ -1309,6 +1266,9 @@ static int run_plan(DeviceState &st, const void *A, const void *B, void *C, size
         p.bias = ea.bias;
         p.c_in = ea.c_in;
         p.c_type = ea.c_type;
+        p.act = ea.act;
+        p.pre = ea.pre;
+        p.in_bf16 = ea.in_bf16;
         if (ea.c_type == kOutF32) p.tma_store = 0;  // FP32 rows leave with plain 16-byte stores
     }
 #ifdef B200_TIMELINE
@@ -1850,7 +1810,9 @@ int b200_hgemm_fused(const void *A, const void *B, void *C, size_t M, size_t N, 
     b200_hgemm_plan pl;
     rc = fused_plan(*st, M, N, K, epilogue->c_type, &pl);
     if (rc != B200_HGEMM_OK) return rc;
-    return run_plan(*st, A, B, C, M, N, K, pl, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, nullptr, epilogue);
+    LibEpilogue epi;
+    static_cast<b200_hgemm_epilogue &>(epi) = *epilogue;
+    return run_plan(*st, A, B, C, M, N, K, pl, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, nullptr, &epi);
 }
 
 int b200_hgemm_fused_ex(const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_hgemm_epilogue *epilogue,
@@ -1863,7 +1825,76 @@ int b200_hgemm_fused_ex(const void *A, const void *B, void *C, size_t M, size_t 
     if (rc != B200_HGEMM_OK) return rc;
     if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
     if (plan->variant == B200_VARIANT_SIMT || plan->variant == B200_VARIANT_CTA2_MCAST) return B200_HGEMM_ERR_UNSUPPORTED;
-    return run_plan(*st, A, B, C, M, N, K, *plan, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, nullptr, epilogue);
+    LibEpilogue epi;
+    static_cast<b200_hgemm_epilogue &>(epi) = *epilogue;
+    return run_plan(*st, A, B, C, M, N, K, *plan, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, nullptr, &epi);
+}
+
+// ---- linear layers --------------------------------------------------------------------------------
+// The dispatch's plan for the shape, as fused_plan gives it. k-ranges summed inside clusters are asked for by name: left
+// to the library they could fall back to a workspace of its own, and this entry point uses the caller's only.
+static int linear_plan(const DeviceState &st, size_t M, size_t N, size_t K, const b200_linear_args &args, b200_hgemm_plan *pl) {
+    const int rc = fused_plan(st, M, N, K, args.c_type, pl);
+    if (rc != B200_HGEMM_OK) return rc;
+    if ((pl->variant == B200_VARIANT_SKINNY || pl->variant == B200_VARIANT_SKINNY_PAIR) && pl->grid == 0 &&
+        skinny_sums_on_chip(*pl, skinny_slices(*pl, st, N, K)) == 1) {
+        pl->grid = 1;
+    }
+    return B200_HGEMM_OK;
+}
+
+static int check_linear(const void *A, const void *B, const void *C, size_t M, size_t N, size_t K, const b200_linear_args *args) {
+    if (!args || !B || N == 0 || K == 0 || (M > 0 && (!A || !C))) return B200_HGEMM_ERR_INVALID_ARG;
+    if (M > 0x7fffff00ull || N > 0x7fffff00ull || K > 0x7fffff00ull) return B200_HGEMM_ERR_UNSUPPORTED;
+    if (args->act < B200_ACT_NONE || args->act > B200_ACT_SILU) return B200_HGEMM_ERR_INVALID_ARG;
+    if (args->in_type != B200_C_F16 && args->in_type != B200_C_BF16) return B200_HGEMM_ERR_INVALID_ARG;
+    if (args->c_type != args->in_type && args->c_type != B200_C_F32) return B200_HGEMM_ERR_INVALID_ARG;
+    if (K % 8 != 0) return B200_HGEMM_ERR_UNSUPPORTED;
+    return B200_HGEMM_OK;
+}
+
+size_t b200_hgemm_linear_workspace_bytes(size_t M, size_t N, size_t K, const b200_linear_args *args) {
+    if (!args || M == 0 || N == 0 || K == 0 || K % 8 != 0) return 0;
+    DeviceState *st = nullptr;
+    static DeviceState nominal;
+    if (current_state(&st) != B200_HGEMM_OK) {
+        cudaGetLastError();
+        nominal.sm_count = 148;
+        st = &nominal;
+    }
+    b200_hgemm_plan pl;
+    if (linear_plan(*st, M, N, K, *args, &pl) != B200_HGEMM_OK) return 0;
+    return b200_hgemm_workspace_bytes(M, N, K, &pl);
+}
+
+int b200_hgemm_linear(const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args *args,
+                      void *workspace, size_t workspace_bytes, b200_stream_t stream) {
+    int rc = check_linear(A, B, C, M, N, K, args);
+    if (rc != B200_HGEMM_OK) return rc;
+    if (M == 0) return B200_HGEMM_OK;
+    DeviceState *st = nullptr;
+    rc = current_state(&st);
+    if (rc != B200_HGEMM_OK) return rc;
+    if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
+    b200_hgemm_plan pl;
+    rc = linear_plan(*st, M, N, K, *args, &pl);
+    if (rc != B200_HGEMM_OK) return rc;
+    const size_t need = b200_hgemm_workspace_bytes(M, N, K, &pl);
+    if (need > 0) {
+        if (!workspace || workspace_bytes < need) return B200_HGEMM_ERR_WORKSPACE;
+        if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200_HGEMM_ERR_MISALIGNED;
+    }
+    LibEpilogue epi;
+    epi.alpha = 1.f;
+    epi.beta = args->residual ? 1.f : 0.f;
+    epi.bias = args->bias;
+    epi.c_in = args->residual;
+    epi.c_type = args->c_type;
+    epi.act = static_cast<uint32_t>(args->act);
+    epi.pre = args->pre;
+    epi.in_bf16 = args->in_type == B200_C_BF16 ? 1u : 0u;
+    return run_plan(*st, A, B, C, M, N, K, pl, reinterpret_cast<cudaStream_t>(stream), need > 0 ? workspace : nullptr, workspace_bytes,
+                    nullptr, &epi);
 }
 
 int b200_hgemm_select(size_t M, size_t N, size_t K, b200_hgemm_plan *plan) {

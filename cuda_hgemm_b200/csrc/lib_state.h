@@ -1,0 +1,85 @@
+// What the library's translation units share: per-device state, the tensor-map cache, launch accounting.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <atomic>
+#include <mutex>
+#include <vector>
+
+namespace b200 {
+
+constexpr int kMaxDevices = 64;
+
+struct TensorMapKey {
+    const void *ptr;
+    uint64_t rows, cols;
+    uint32_t box_rows, box_cols;
+    bool swizzle;
+    uint64_t batch, batch_stride;  // stacks of matrices: how many, and elements from one to the next (1, 0: a single matrix)
+    uint32_t elem_bytes;           // 2: 16-bit elements of either kind (a copy does not tell them apart), 4: FP32
+    bool operator==(const TensorMapKey &o) const {
+        return ptr == o.ptr && rows == o.rows && cols == o.cols && box_rows == o.box_rows && box_cols == o.box_cols &&
+               swizzle == o.swizzle && batch == o.batch && batch_stride == o.batch_stride && elem_bytes == o.elem_bytes;
+    }
+};
+
+struct TensorMapSlot {
+    bool used = false;
+    uint64_t last_use = 0;
+    TensorMapKey key{};
+    CUtensorMap map{};
+};
+constexpr size_t kTensorMapWays = 4;
+
+struct DeviceState {
+    std::mutex mu;
+    bool probed = false;       // attributes known and the error word allocated
+    bool attrs_known = false;  // sm100 / sm_count filled in (no allocation needed for that)
+    bool sm100 = false;
+    int sm_count = 0;
+    uint32_t *error_word = nullptr;
+    // stream-k workspace [64 KiB header | FP32 partial slots]: either one the caller handed over
+    // (ws), or one per stream that the library allocates and grows itself, so that GEMMs running
+    // on different streams at the same time never share partial-tile slots
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+    struct StreamWorkspace {
+        cudaStream_t stream;
+        void *ptr;
+        size_t bytes;
+        uint64_t last_use;
+    };
+    std::vector<StreamWorkspace> owned_ws;
+    uint64_t ws_clock = 0;
+    // staging buffers of the host-pointer entry point
+    void *host_a = nullptr, *host_b = nullptr, *host_c = nullptr;
+    size_t host_a_bytes = 0, host_b_bytes = 0, host_c_bytes = 0;
+    cudaStream_t host_stream[3] = {nullptr, nullptr, nullptr};  // upload, GEMMs, download
+    cudaEvent_t host_event[2] = {nullptr, nullptr};
+    bool attr_set[128] = {};    // slots from 96 on: the grouped kernels
+    int max_clusters[128] = {};
+    int ck_clusters[16][9] = {};  // short-A kernels that sum inside clusters: clusters of each size the device holds at once (-1: none)  // CTA pairs the device can keep resident at once, per pair kernel
+    TensorMapSlot tm_cache[64 * kTensorMapWays];
+    uint64_t tm_clock = 0;
+};
+
+extern std::atomic<uint64_t> g_launches;
+
+// Logs a failing CUDA call when B200_HGEMM_DEBUG is set; true on success.
+bool cuda_ok(cudaError_t e, const char *what);
+// State of the current device, probed on first use (a status on failure).
+int current_state(DeviceState **out);
+// The tensor map of a row-major matrix (or stack of matrices) viewed through boxes, from the cache or encoded.
+int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
+                   CUtensorMap *out, bool swizzle = true, uint64_t batch = 1, uint64_t batch_stride = 0, uint32_t elem_bytes = 2);
+bool pdl_enabled();
+
+inline uint32_t ceil_div_u32(uint64_t a, uint64_t b) {
+    return static_cast<uint32_t>((a + b - 1) / b);
+}
+
+}  // namespace b200

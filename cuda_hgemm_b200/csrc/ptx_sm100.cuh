@@ -265,6 +265,14 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *tm, uint32_t sme
                  : "memory");
 }
 
+// Adds the box to what is in global memory, element by element, in the tensor map's type.
+__device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap *tm, uint32_t smem_src, int32_t x, int32_t y, int32_t z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 :
+                 : "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+
 __device__ __forceinline__ void tma_store_commit() {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -364,6 +372,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16_f32(uint32_t m, uint32_t n
 __host__ __device__ constexpr uint32_t umma_idesc_f16_f32_b_mn(uint32_t m, uint32_t n) {
     return umma_idesc_f16_f32(m, n) | (1u << 16);
 }
+
+// Added to any of these: A and B are BF16 (format 1 in both fields; the two always agree here).
+constexpr uint32_t kUmmaIdescBf16 = (1u << 7) | (1u << 10);
+// Added: the A operand is MN-major (bit 15).
+constexpr uint32_t kUmmaIdescAMn = 1u << 15;
 
 // D[tmem] (+)= A[smem] * B[smem]; issued by ONE thread.
 template <int kCtaGroup>

@@ -177,6 +177,68 @@ int b200_hgemm_bkn(const void *A, const void *B_kn, void *C, size_t M, size_t N,
 int b200_hgemm_batched(const void *A, const void *B, void *C, size_t M, size_t N, size_t K, size_t batch,
                        size_t stride_a, size_t stride_b, size_t stride_c, b200_stream_t stream);
 
+/* ---- the products of a feed-forward layer: dense and by expert, forward and backward -----------------------
+ * No counterpart in the reference (one product, FP16, nothing after it: src/main.cu:11). With A [M x K],
+ * B [N x K], C [M x N], all row-major, inputs FP16 or BF16, sums in FP32:
+ *
+ *   forward    Z = A * B^T + bias          C = act(Z) + residual
+ *   backward   dZ = dC .* act'(Z)          dA = dZ * B      dB = dZ^T * A      dbias = column sums of dZ
+ *
+ * The grouped forms multiply the rows [offsets[g], offsets[g+1]) of A by their own matrix B_g: `offsets` holds G + 1
+ * int32 values in DEVICE memory, ascending within [0, M], so that whatever counted the rows never has to come back to
+ * the host. Groups may be empty (their dB and dbias are zeros); rows before offsets[0] and from offsets[G] on belong
+ * to no group: their rows of C, Z, dZ and dA are neither computed nor written. Offsets out of order or out of range
+ * give undefined results but no access outside the operands. M = 0 is allowed everywhere here (there is nothing
+ * to write but zero gradients).
+ *
+ * Scratch: only what the caller passes (256-byte aligned; the *_workspace_bytes functions say how much, often
+ * none), nothing is allocated or kept, so calls on different streams and captured graphs never share any. */
+enum {
+    B200_ACT_NONE = 0,
+    B200_ACT_RELU = 1,
+    B200_ACT_GELU = 2,      /* z * Phi(z), by the error function */
+    B200_ACT_GELU_TANH = 3, /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+    B200_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+};
+typedef struct b200_linear_args {
+    int32_t in_type;      /* B200_C_F16 or B200_C_BF16: type of A, B and bias */
+    int32_t c_type;       /* type of C, residual and pre: in_type, or B200_C_F32 */
+    int32_t act;          /* B200_ACT_* */
+    const void *bias;     /* N values (grouped: G x N), or NULL */
+    const void *residual; /* M x N, may be C itself, or NULL; the grouped form takes none (B200_HGEMM_ERR_UNSUPPORTED) */
+    void *pre;            /* M x N: receives Z, for the backward pass; or NULL */
+} b200_linear_args;
+/* The dispatch is that of b200_hgemm; K % 8 == 0, any N. */
+int b200_hgemm_linear(const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args *args,
+                      void *workspace, size_t workspace_bytes, b200_stream_t stream);
+size_t b200_hgemm_linear_workspace_bytes(size_t M, size_t N, size_t K, const b200_linear_args *args);
+/* B: G matrices, stride_b elements apart (a multiple of 8, at least N * K). G <= 1024. K % 8 == 0, any N. No workspace. */
+int b200_hgemm_grouped(const void *A, const void *B, void *C, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
+                       size_t stride_b, const b200_linear_args *args, b200_stream_t stream);
+
+typedef struct b200_linear_grads {
+    int32_t in_type;    /* type of A, B, dA and dZ */
+    int32_t c_type;     /* type of dC and pre: in_type, or B200_C_F32 */
+    int32_t act;        /* B200_ACT_* of the forward pass */
+    int32_t db_type;    /* type of dB: in_type, or B200_C_F32 */
+    int32_t accumulate; /* 1: dB and dbias are added to (dB must be B200_C_F32); 0: overwritten */
+    const void *dC;     /* M x N */
+    const void *pre;    /* M x N: the forward pass's Z; may be NULL when act is B200_ACT_NONE */
+    void *dZ;           /* M x N: receives dZ (rounded to in_type, as the products read it), may be dC when the types
+                         * agree; NULL: kept in the workspace where it is needed */
+    void *dA;           /* M x K, or NULL: not wanted */
+    void *dB;           /* N x K (grouped: G x N x K, dense), or NULL */
+    float *dbias;       /* N (grouped: G x N) FP32 sums of the unrounded dZ, or NULL */
+} b200_linear_grads;
+/* K % 8 == 0 and N % 8 == 0. A may be NULL without dB, B may be NULL without dA. The gradient of the residual is dC. */
+int b200_hgemm_linear_backward(const void *A, const void *B, size_t M, size_t N, size_t K, const b200_linear_grads *grads,
+                               void *workspace, size_t workspace_bytes, b200_stream_t stream);
+int b200_hgemm_grouped_backward(const void *A, const void *B, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
+                                size_t stride_b, const b200_linear_grads *grads, void *workspace, size_t workspace_bytes,
+                                b200_stream_t stream);
+/* G = 1 for the dense form. */
+size_t b200_hgemm_backward_workspace_bytes(size_t M, size_t N, size_t K, size_t G, const b200_linear_grads *grads);
+
 /* HOST-pointer GEMM: copies A and B to the device, runs b200_hgemm, copies C back and
  * synchronises. This is the path of reference Matrix (src/common/matrix.h:23-35 upload,
  * :83-85 moveToHost) + one kernel call, behind one entry point. Returns after C_host is complete. */
