@@ -82,13 +82,9 @@ struct alignas(64) GemmParams {
     uint32_t c_vec_ok;   // 1: 16-byte vector stores to C are aligned (N % 8 == 0)
     // fused epilogue (kernels instantiated with EPI only): C = alpha * A*B^T + beta * c_in + bias
     float alpha, beta;
-    const __half *bias;  // N values (BF16 with in_bf16), one per column of C, or nullptr
+    const __half *bias;  // N values, one per column of C, or nullptr
     const void *c_in;    // M x N of C's element type, row-major, read when beta != 0 (may be C itself), or nullptr
     uint32_t c_type;     // OutType of C and c_in (kernels with the fused epilogue only; 0 = FP16)
-    // linear layers: C = act(Z) + beta * c_in with Z = alpha * A*B^T + bias, Z kept in `pre` when that is set
-    void *pre;           // M x N of C's element type, or nullptr
-    uint32_t act;        // ActKind
-    uint32_t in_bf16;    // A, B and bias are BF16
     // Tail of a launch with larger tiles (whole-tile mode only; tail_sm = 0: off). This launch's tile u is part
     // u % (tail_sm * tail_sn) of the larger tile tail_first + u / (tail_sm * tail_sn), which is located with
     // the larger tiles' own geometry and split tail_sm x tail_sn ways.
@@ -255,19 +251,16 @@ struct EpilogueArgs {
     const __half *bias;  // BF16 with in_bf16
     const void *c_in;
     uint32_t c_type;
+    // linear layers (short-A kernels only): C = act(Z) + beta * c_in, Z = alpha * A*B^T + bias
     uint32_t act;      // ActKind
-    void *pre;         // M x N of C's type: receives the value before the activation, or null
+    void *pre;         // M x N of C's type: receives Z, or null
     uint32_t in_bf16;  // A, B and bias are BF16
 };
-
-__device__ __forceinline__ float load_bias(const __half *bias, uint32_t col, uint32_t bf16) {
-    return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(bias)[col]) : __half2float(bias[col]);
-}
 
 // v = act(alpha * v + bias[col]) + beta * c_in[row][col] for one element (callers check the bounds).
 __device__ __forceinline__ float fused_value(const EpilogueArgs &e, float acc, size_t row, uint32_t col, uint32_t n) {
     float v = e.alpha * acc;
-    if (e.bias) v += load_bias(e.bias, col, e.in_bf16);
+    if (e.bias) v += e.in_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(e.bias)[col]) : __half2float(e.bias[col]);
     if (e.pre) store_c_elem(e.pre, row * n + col, v, e.c_type);
     if (e.act != kActNone) {
         uint32_t bits = __float_as_uint(v);
@@ -278,25 +271,9 @@ __device__ __forceinline__ float fused_value(const EpilogueArgs &e, float acc, s
     return v;
 }
 
-// Eight FP32 values of one row -> C's element type -> 32 or 16 aligned bytes of global memory.
-__device__ __forceinline__ void store_c8(void *base, size_t i, const float (&v)[8], uint32_t c_type) {
-    if (c_type == kOutF32) {
-        float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(base) + i);
-        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-        return;
-    }
-    uint4 w;
-    w.x = pack2_rn(__float_as_uint(v[0]), __float_as_uint(v[1]), c_type);
-    w.y = pack2_rn(__float_as_uint(v[2]), __float_as_uint(v[3]), c_type);
-    w.z = pack2_rn(__float_as_uint(v[4]), __float_as_uint(v[5]), c_type);
-    w.w = pack2_rn(__float_as_uint(v[6]), __float_as_uint(v[7]), c_type);
-    *reinterpret_cast<uint4 *>(static_cast<__half *>(base) + i) = w;
-}
-
 // Fused epilogue on COUNT accumulator columns of one row, in place (FP32 bit patterns):
-// v = act(alpha * v + bias[col]) + beta * c_in[row][col], the value before the activation stored on the way when
-// it is wanted. Out-of-range rows and columns are left alone (they are clipped when stored).
+// v = alpha * v + bias[col] + beta * c_in[row][col]. Out-of-range rows and columns are left alone
+// (they are clipped when stored).
 template <int COUNT>
 __device__ __forceinline__ void fused_epilogue(const GemmParams &p, uint32_t row, uint32_t col0, uint32_t *vals) {
     const bool row_ok = row < p.m;
@@ -304,61 +281,16 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams &p, uint32_t row
     const __half *bias = p.bias ? p.bias + col0 : nullptr;
     const bool use_cin = p.beta != 0.f && p.c_in && row_ok;
     const size_t cin_off = static_cast<size_t>(row) * p.n + col0;
-    const bool linear = p.act != kActNone || p.pre != nullptr;  // uniform over the launch
-    if (linear) {
-        // Z first, in place; what follows then has the residual alone to add
-#pragma unroll
-        for (int j = 0; j < COUNT; j += 8) {
-            float z[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = p.alpha * __uint_as_float(vals[j + e]);
-            if (bias) {
-                if (vec_ok) {
-                    const uint4 b = *reinterpret_cast<const uint4 *>(bias + j);
-                    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = p.in_bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]))
-                                                   : __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-                        z[2 * e] += f.x;
-                        z[2 * e + 1] += f.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (col0 + j + e < p.n) z[e] += load_bias(bias, j + e, p.in_bf16);
-                    }
-                }
-            }
-            if (p.pre && row_ok) {
-                if (vec_ok) {
-                    store_c8(p.pre, cin_off + j, z, p.c_type);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (col0 + j + e < p.n) store_c_elem(p.pre, cin_off + j + e, z[e], p.c_type);
-                    }
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) vals[j + e] = __float_as_uint(z[e]);
-        }
-        act_apply<COUNT>(vals, p.act);
-        if (!use_cin) return;
-        bias = nullptr;
-    }
-    const float scale = linear ? 1.f : p.alpha;
 #pragma unroll
     for (int j = 0; j < COUNT; j += 8) {
         float add[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (vec_ok) {
             if (bias) {
                 const uint4 b = *reinterpret_cast<const uint4 *>(bias + j);
-                const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+                const __half2 *h = reinterpret_cast<const __half2 *>(&b);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float2 f = p.in_bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]))
-                                               : __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+                    const float2 f = __half22float2(h[e]);
                     add[2 * e] += f.x;
                     add[2 * e + 1] += f.y;
                 }
@@ -394,13 +326,13 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams &p, uint32_t row
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (col0 + j + e < p.n) {
-                    if (bias) add[e] += load_bias(bias, j + e, p.in_bf16);
+                    if (bias) add[e] += __half2float(bias[j + e]);
                     if (use_cin) add[e] += p.beta * load_c_elem(p.c_in, cin_off + j + e, p.c_type);
                 }
             }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vals[j + e] = __float_as_uint(fmaf(scale, __uint_as_float(vals[j + e]), add[e]));
+        for (int e = 0; e < 8; ++e) vals[j + e] = __float_as_uint(fmaf(p.alpha, __uint_as_float(vals[j + e]), add[e]));
     }
 }
 
@@ -639,8 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_tcgen05_kernel(const __grid
         // ------------------------------------------------------------------ MMA issuer
         if (lane == 0 && cta_rank == 0) {
             constexpr uint32_t kMmaN = T::kWide ? BN / 2 : BN;  // columns one MMA writes
-            constexpr uint32_t idesc_f16 = BKN ? umma_idesc_f16_f32_b_mn(kBM * CG, kMmaN) : umma_idesc_f16_f32(kBM * CG, kMmaN);
-            const uint32_t idesc = EPI && p.in_bf16 ? idesc_f16 | kUmmaIdescBf16 : idesc_f16;
+            constexpr uint32_t idesc = BKN ? umma_idesc_f16_f32_b_mn(kBM * CG, kMmaN) : umma_idesc_f16_f32(kBM * CG, kMmaN);
             WorkWalker<MODE> work(p, worker, workers);
             Segment seg;
             uint32_t stage = 0, phase = 0, it = 0;

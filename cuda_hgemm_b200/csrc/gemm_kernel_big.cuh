@@ -154,7 +154,7 @@ __device__ __forceinline__ void hgemm_big_body(const GemmParams &p) {
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer (pair leaders)
         if (lane == 0 && half == 0) {
-            const uint32_t idesc = umma_idesc_f16_f32(256, BN) | (EPI && p.in_bf16 ? kUmmaIdescBf16 : 0u);
+            constexpr uint32_t idesc = umma_idesc_f16_f32(256, BN);
             const uint16_t pair_mask = static_cast<uint16_t>(quad ? (0x3u << (2u * pair)) : 0x3u);
             const uint16_t all_mask = static_cast<uint16_t>(quad ? 0xFu : 0x3u);
             uint32_t stage = 0, phase = 0;

@@ -11,9 +11,16 @@
 // lane = output column, tensor-memory column = row of the group. An MMA's column count is chosen at run
 // time in steps of 16 (32 for a pair), so a group of 300 rows is two blocks of 160 and 140, where the other
 // way round it would be three blocks of 128 (or two of 256 on a pair) filled to 78 (59) percent; a group of three
-// rows costs an MMA of 16 columns and stages 16 rows. The rows' operand is staged by at most four copies out of
-// boxes of 128, 64, 32 and 16 rows. The weight gradient sums over the group's rows: both operands
-// are then row-contiguous in the other index and read by the MMA as MN-major; the accumulator is not transposed.
+// rows costs an MMA of 16 columns and stages 16 rows. The rows' operand has a tensor map for every height of a
+// block (16 to 128 rows), so that one copy stages it: putting a block together from boxes of 128, 64, 32 and 16
+// rows kept the thread that issues the copies busy for longer than the MMAs last (8192 x 8192 x 8192 in one group:
+// 904 us against 797). The weight gradient sums over the group's rows: both operands are then row-contiguous in the
+// other index and read by the MMA as MN-major; the accumulator is not transposed.
+//
+// FP32 results of long sums (LONG): the tensor cores cut off what an accumulator cannot hold instead of rounding
+// it, a relative 1.7e-6 after 128 MMAs (a sum of 2048) and growing with the length. That is nothing next to
+// a 16-bit result's rounding, but 30 times FP32's own. Those sums are cut into pieces of kLongBlocks k-blocks that
+// alternate between the two accumulators, and the epilogue warps add the pieces in registers, rounding to nearest.
 //
 // Group sizes are known on the device only (a router wrote them): every CTA reads the offsets, cuts the groups
 // into tiles and walks its share of them. Offsets that are out of order or past T are held within [0, T].
@@ -31,6 +38,7 @@
 #include <cuda_bf16.h>
 
 #include "activation.cuh"
+#include "lib_state.h"
 #include "ptx_sm100.cuh"
 #include "sched.h"
 
@@ -42,17 +50,21 @@ enum GroupedForm : int {
     kFormWeight = 2,
 };
 
-constexpr int kGroupedThreads = 192;
+constexpr int kGroupedEpiWarps = 8;
+constexpr int kGroupedThreads = 64 + 32 * kGroupedEpiWarps;
+constexpr uint32_t kLongBlocks = kLongSum / 64;  // k-blocks summed by the tensor cores before the piece is added up in FP32
 constexpr uint32_t kGroupedMaxGroups = 1024;
 constexpr uint32_t kGroupedBand = 8;  // blocks of rows a band of tiles is high
 
 struct alignas(64) GroupedParams {
-    CUtensorMap tm_p;     // forward {K, N, groups} box {64, 128}; input {K, N, groups} box {64, 64}; weight {N, T} box {64, 64}
-    CUtensorMap tm_q[4];  // forward {K, T}, input {N, T}: boxes {64, 128 >> i}; weight: [0] = {K, T} box {64, 64}
+    CUtensorMap tm_p;     // forward {K, N, groups} box {64, 128}; input {K, N, groups} box {64, 64}; weight {N, T} box {64, 64} or
+                          // {64, T, N / 64} box {64, 64, 2}
+    CUtensorMap tm_q[8];  // forward {K, T}, input {N, T}: boxes {64, 16 (i + 1)}; weight: [0] = {K, T} as P
     CUtensorMap tm_out;   // weight: {K, N, groups}, box of 128 bytes x 32 rows
     void *out;
     void *pre;             // forward: Z = sum + bias before the activation, or null
     const void *bias;      // forward: groups x N of the inputs' type, or null
+    const void *residual;  // forward: T x N of C's type, added behind the activation, or null
     const int32_t *offsets;  // groups + 1, or null: one group of all rows
     uint32_t *error_word;
     uint32_t rows;         // T
@@ -67,29 +79,33 @@ struct alignas(64) GroupedParams {
     uint32_t out_type;     // 0 FP16, 1 BF16, 2 FP32
     uint32_t act;
     uint32_t accumulate;   // weight, FP32: add to the output
+    uint32_t p_wide, q_wide;  // weight: the operand's map takes two boxes with one copy (load_columns)
     FastDiv p_div;         // by p_blocks
 };
 
-template <int FORM, int CG, int QT, int STAGES, int KPS>
+template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG>
 struct GroupedTraits {
     static constexpr bool kWeight = FORM == kFormWeight;
     static_assert(CG == 1 || CG == 2, "single CTAs or CTA pairs");
     static_assert(QT == 32 || QT == 64 || QT == 128 || QT == 256, "columns of an accumulator");
     static_assert(!kWeight || (QT / CG == 128 && KPS == 1), "weight form: two 64-column boxes of Q per CTA");
+    static_assert(!LONG || FORM != kFormInput, "the input's gradient is 16-bit");
+    static_assert(kLongBlocks % KPS == 0, "whole stages per piece of a long sum");
+    static constexpr uint32_t kChunk = QT >= 64 ? 32 : 16;  // accumulator columns an epilogue warp takes at a time
     static constexpr uint32_t kStep = 16u * CG;  // an MMA's columns come in these steps
     static constexpr uint32_t kPBytes = 128u * 128u;
     static constexpr uint32_t kQBytes = (QT / CG) * 128u;
     static constexpr uint32_t kBlockBytes = kPBytes + kQBytes;
     static constexpr uint32_t kStageBytes = KPS * kBlockBytes;
     static constexpr uint32_t kTmemCols = 2u * QT;
-    static constexpr uint32_t kStagingBytes = kWeight ? 4u * 2u * 4096u : 0u;
+    static constexpr uint32_t kStagingBytes = kWeight ? kGroupedEpiWarps * 4096u : 0u;
     static constexpr uint32_t kTableBytes = kWeight ? 0u : 2u * 4u * (kGroupedMaxGroups + 4u);
     static constexpr uint32_t kBarrierBytes = 256;
     static constexpr uint32_t kSmemBytes = 1024 + STAGES * kStageBytes + kStagingBytes + kTableBytes + kBarrierBytes;
     static_assert(kBlockBytes % 1024 == 0, "operand slabs must keep 1024-byte alignment");
     static_assert(kSmemBytes <= 232448, "exceeds 227 KB of shared memory");
     static_assert((kWeight ? 32u : 16u) * STAGES + 40u <= kBarrierBytes, "barrier area too small");
-    static_assert(QT / CG <= 128, "rows of Q a CTA stages: one box of 128 and the smaller ones");
+    static_assert(QT / CG <= 128, "rows of Q a CTA stages: the highest box has 128");
     static_assert(STAGES <= 16, "one lane of a warp per barrier to set up");
 };
 
@@ -169,8 +185,24 @@ __device__ __forceinline__ void weight_tile(const GroupedParams &p, uint32_t t, 
     out.p0 = pb * 128u * CG;
     out.q0 = qb * QT;
     out.valid = end - start;
-    out.n_mma = min(static_cast<uint32_t>(QT), round_up_u32(p.q_dim - out.q0, 16u * CG));
+    out.n_mma = min(static_cast<uint32_t>(QT), round_up_u32(p.q_dim - out.q0, 64u * CG));  // whole 64-column boxes per CTA
     out.row0 = start;
+}
+
+// Weight form: 64 rows of 128 columns from column x (a multiple of 64) on, as two boxes of 64 columns one behind the other. A matrix
+// whose width is a multiple of 64 is mapped as {64, rows, width / 64}, where one copy takes both (`wide`): issuing
+// the copies is what the producer's one thread spends its time on.
+template <bool PAIR>
+__device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap &map, uint32_t wide, int32_t x, int32_t row, uint32_t bar) {
+    if (wide) {
+        if (PAIR) tma_load_3d_pair(dst, &map, 0, row, x >> 6, bar); else tma_load_3d(dst, &map, 0, row, x >> 6, bar);
+    } else if (PAIR) {
+        tma_load_2d_pair(dst, &map, x, row, bar);
+        tma_load_2d_pair(dst + 8192u, &map, x + 64, row, bar);
+    } else {
+        tma_load_2d(dst, &map, x, row, bar);
+        tma_load_2d(dst + 8192u, &map, x + 64, row, bar);
+    }
 }
 
 // An mbarrier wait that also acquires what other CTAs of the cluster wrote before they arrived.
@@ -196,16 +228,17 @@ __device__ __forceinline__ uint32_t pack2_typed(uint32_t lo_f32_bits, uint32_t h
     return pack_half2_rn(lo_f32_bits, hi_f32_bits);
 }
 
-// A 32-column chunk of a transposed accumulator (this lane: output column `col`, register j: row q0 + j) to
+// COUNT columns of a transposed accumulator (this lane: output column `col`, register j: row q0 + j) to
 // row-major memory. 16-bit outputs whose rows are a whole number of 4-byte words leave two columns at a
 // time: neighbouring lanes exchange halves, the even lane takes the even rows and the odd lane the odd rows,
 // so that a warp stores two rows of 64 bytes with one instruction instead of one.
-__device__ __forceinline__ void store_transposed32(void *out, uint32_t out_type, uint32_t q0, uint32_t valid, uint32_t col,
-                                                   uint32_t dim, const uint32_t (&r)[32], uint32_t lane) {
+template <int COUNT>
+__device__ __forceinline__ void store_transposed(void *out, uint32_t out_type, uint32_t q0, uint32_t valid, uint32_t col,
+                                                 uint32_t dim, const uint32_t *r, uint32_t lane) {
     if (out_type == 2u) {
         float *dst = static_cast<float *>(out) + static_cast<size_t>(q0) * dim + col;
 #pragma unroll
-        for (uint32_t j = 0; j < 32; ++j) {
+        for (uint32_t j = 0; j < COUNT; ++j) {
             if (j < valid && col < dim) dst[static_cast<size_t>(j) * dim] = __uint_as_float(r[j]);
         }
         return;
@@ -214,7 +247,7 @@ __device__ __forceinline__ void store_transposed32(void *out, uint32_t out_type,
         const uint32_t odd = lane & 1u;
         uint32_t *dst = static_cast<uint32_t *>(out) + ((static_cast<size_t>(q0) + odd) * dim + (col & ~1u)) / 2u;
 #pragma unroll
-        for (uint32_t j = 0; j < 32; j += 2) {
+        for (uint32_t j = 0; j < COUNT; j += 2) {
             const uint32_t mine = pack2_typed(r[j], r[j + 1], out_type);  // rows j and j + 1 of this column
             const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
             // even lane: row j of (this, next) column; odd lane: row j + 1 of (previous, this)
@@ -225,14 +258,54 @@ __device__ __forceinline__ void store_transposed32(void *out, uint32_t out_type,
     }
     unsigned short *dst = static_cast<unsigned short *>(out) + static_cast<size_t>(q0) * dim + col;
 #pragma unroll
-    for (uint32_t j = 0; j < 32; ++j) {
+    for (uint32_t j = 0; j < COUNT; ++j) {
         if (j < valid && col < dim) dst[static_cast<size_t>(j) * dim] = static_cast<unsigned short>(pack2_typed(r[j], r[j], out_type));
     }
 }
 
-template <int FORM, int CG, int QT, int STAGES, int KPS>
+// Adds the residual's values at the same places. All of them are read before any is stored over (it may be C itself).
+template <int COUNT>
+__device__ __forceinline__ void add_residual(const void *residual, uint32_t type, uint32_t q0, uint32_t valid, uint32_t col,
+                                             uint32_t dim, uint32_t *r) {
+    const size_t at = static_cast<size_t>(q0) * dim + col;
+#pragma unroll
+    for (uint32_t j = 0; j < COUNT; ++j) {
+        if (j < valid && col < dim) {
+            const size_t i = at + static_cast<size_t>(j) * dim;
+            const float v = type == 2u ? static_cast<const float *>(residual)[i]
+                            : type == 1u ? __bfloat162float(static_cast<const __nv_bfloat16 *>(residual)[i])
+                                         : __half2float(static_cast<const __half *>(residual)[i]);
+            r[j] = __float_as_uint(__uint_as_float(r[j]) + v);
+        }
+    }
+}
+
+// What becomes of COUNT columns of an accumulator of the forward or input form.
+template <int FORM, int COUNT>
+__device__ __forceinline__ void finish_rows(const GroupedParams &p, uint32_t *r, float bias, uint32_t q0, uint32_t valid, uint32_t col,
+                                            uint32_t lane) {
+    if (FORM == kFormForward) {
+        if (p.bias) {
+#pragma unroll
+            for (uint32_t j = 0; j < COUNT; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + bias);
+        }
+        if (p.pre) store_transposed<COUNT>(p.pre, p.out_type, q0, valid, col, p.p_dim, r, lane);
+        act_apply<COUNT>(r, p.act);
+        if (p.residual) add_residual<COUNT>(p.residual, p.out_type, q0, valid, col, p.p_dim, r);
+    }
+    store_transposed<COUNT>(p.out, p.out_type, q0, valid, col, p.p_dim, r, lane);
+}
+
+// COUNT (16 or 32) accumulator columns of this lane's row.
+template <int COUNT>
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t *r) {
+    if (COUNT == 32) tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
+    else tmem_ld_32x32b_x16(taddr, *reinterpret_cast<uint32_t(*)[16]>(r));
+}
+
+template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG>
 __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const __grid_constant__ GroupedParams p) {
-    using T = GroupedTraits<FORM, CG, QT, STAGES, KPS>;
+    using T = GroupedTraits<FORM, CG, QT, STAGES, KPS, LONG>;
     constexpr bool WEIGHT = FORM == kFormWeight;
     constexpr bool P_MN = FORM != kFormForward;  // P is read MN-major
     constexpr uint32_t kStepK = 64u;             // summed index per k-block
@@ -272,7 +345,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
         } else if (lane < static_cast<uint32_t>(STAGES) + 2u) {
             const uint32_t a = lane - STAGES;
             mbar_init(tfull_bar + 8u * a, 1);
-            mbar_init(tempty_bar + 8u * a, 4 * CG);
+            mbar_init(tempty_bar + 8u * a, kGroupedEpiWarps * CG);
         } else if (lane == static_cast<uint32_t>(STAGES) + 2u) {
             *abort_flag = 0;
         }
@@ -344,24 +417,19 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 const uint32_t q_rows = tile.n_mma / CG;  // forward, input: rows this CTA stages
                 const int32_t p_at = static_cast<int32_t>(tile.p0 + cta_rank * 128u);
                 const int32_t q_at = static_cast<int32_t>(tile.q0 + cta_rank * q_rows);
+                const CUtensorMap *q_map = &p.tm_q[WEIGHT ? 0u : q_rows / 16u - 1u];
                 const uint32_t bytes = KPS * (T::kPBytes + (WEIGHT ? T::kQBytes : q_rows * 128u));
-                for (uint32_t kb = 0; kb < blocks; ++kb) {
+                const uint32_t rest = WEIGHT ? (tile.valid & (kStepK - 1u)) : 0u;  // rows of a tail, 0: whole blocks
+                const uint32_t whole = blocks - (rest != 0 ? 1u : 0u);
+                for (uint32_t kb = 0; kb < whole; ++kb) {
                     if (!mbar_wait(empty_bar + 8u * stage, phase ^ 1u, abort_flag)) {
                         ok = false;
                         break;
                     }
                     const uint32_t slot = base + stage * T::kStageBytes;
-                    // the last block of a group that does not fill it: its lines are cleared behind the group's end
-                    const bool tail = WEIGHT && kb + 1u == blocks && (tile.valid & (kStepK - 1u)) != 0;
-                    // A pair's copies complete on the leader's barrier, which expects the bytes of both; a tail's on
-                    // the barrier of the CTA whose MMA warp clears its part.
-                    const bool pair = CG == 2 && !tail;
                     uint32_t bar = full_bar + 8u * stage;
-                    if (CG == 2 && tail) {
-                        if (cta_rank == 0) mbar_arrive(bar);  // keeps the stage's phase; nothing is waited for there
-                        bar = tail_bar + 8u * stage;
-                        mbar_arrive_expect_tx(bar, bytes);
-                    } else if (CG == 2) {
+                    if (CG == 2) {
+                        // both CTAs' copies complete on the leader's barrier, which expects the bytes of both
                         if (cta_rank == 0) mbar_arrive_expect_tx(bar, 2u * bytes);
                         bar = map_to_cta(bar, 0);
                     } else {
@@ -374,40 +442,44 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                         const int32_t kx = static_cast<int32_t>((kb * KPS + j) * kStepK);  // past the end: zeros in both operands
                         if (WEIGHT) {
                             const int32_t row = static_cast<int32_t>(tile.row0) + kx;
-#pragma unroll
-                            for (int32_t h = 0; h < 2; ++h) {
-                                if (pair) {
-                                    tma_load_2d_pair(sp + h * 8192u, &p.tm_p, p_at + h * 64, row, bar);
-                                    tma_load_2d_pair(sq + h * 8192u, &p.tm_q[0], q_at + h * 64, row, bar);
-                                } else {
-                                    tma_load_2d(sp + h * 8192u, &p.tm_p, p_at + h * 64, row, bar);
-                                    tma_load_2d(sq + h * 8192u, &p.tm_q[0], q_at + h * 64, row, bar);
-                                }
-                            }
+                            load_columns<CG == 2>(sp, p.tm_p, p.p_wide, p_at, row, bar);
+                            load_columns<CG == 2>(sq, p.tm_q[0], p.q_wide, q_at, row, bar);
                         } else {
                             const int32_t g = static_cast<int32_t>(tile.group);
                             if (FORM == kFormForward) {
-                                if (pair) tma_load_3d_pair(sp, &p.tm_p, kx, p_at, g, bar); else tma_load_3d(sp, &p.tm_p, kx, p_at, g, bar);
+                                if (CG == 2) tma_load_3d_pair(sp, &p.tm_p, kx, p_at, g, bar); else tma_load_3d(sp, &p.tm_p, kx, p_at, g, bar);
                             } else {
 #pragma unroll
                                 for (int32_t h = 0; h < 2; ++h) {
-                                    if (pair) tma_load_3d_pair(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
+                                    if (CG == 2) tma_load_3d_pair(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
                                     else tma_load_3d(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
                                 }
                             }
-                            uint32_t done = 0;
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) {
-                                const uint32_t box = 128u >> i;
-                                if (box <= static_cast<uint32_t>(QT / CG) && q_rows - done >= box) {
-                                    const int32_t y = q_at + static_cast<int32_t>(done);
-                                    if (pair) tma_load_2d_pair(sq + done * 128u, &p.tm_q[i], kx, y, bar);
-                                    else tma_load_2d(sq + done * 128u, &p.tm_q[i], kx, y, bar);
-                                    done += box;
-                                }
-                            }
+                            if (CG == 2) tma_load_2d_pair(sq, q_map, kx, q_at, bar); else tma_load_2d(sq, q_map, kx, q_at, bar);
                         }
                     }
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (WEIGHT && ok && rest != 0) {
+                    // the last block of a group that does not fill it: the MMA warp of each CTA clears its lines behind the
+                    // group's end, so in a pair each CTA's copies complete on a barrier of its own
+                    if (!mbar_wait(empty_bar + 8u * stage, phase ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sp = base + stage * T::kStageBytes;
+                    uint32_t bar = full_bar + 8u * stage;
+                    if (CG == 2) {
+                        if (cta_rank == 0) mbar_arrive(bar);  // keeps the stage's phase; nothing lands there
+                        bar = tail_bar + 8u * stage;
+                    }
+                    mbar_arrive_expect_tx(bar, bytes);
+                    const int32_t row = static_cast<int32_t>(tile.row0 + whole * kStepK);
+                    load_columns<false>(sp, p.tm_p, p.p_wide, p_at, row, bar);
+                    load_columns<false>(sp + T::kPBytes, p.tm_q[0], p.q_wide, q_at, row, bar);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -432,14 +504,26 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 const uint32_t blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks;
                 if (blocks == 0) continue;
                 const uint32_t rest = WEIGHT ? (tile.valid & (kStepK - 1u)) : 0u;  // rows of a tail, 0: whole blocks
-                const uint32_t acc = it & 1u;
-                const uint32_t d_tmem = tmem_base + acc * QT;
                 const uint32_t idesc = idesc_base | ((tile.n_mma >> 3) << 17);
+                const uint32_t whole = blocks - (rest != 0 ? 1u : 0u);
+                uint32_t d_tmem = tmem_base + (it & 1u) * QT;
                 if (cta_rank == 0 && lane == 0) {
-                    if (!mbar_wait(tempty_bar + 8u * acc, ((it >> 1) & 1u) ^ 1u, abort_flag)) ok = false;
+                    if (!mbar_wait(tempty_bar + 8u * (it & 1u), ((it >> 1) & 1u) ^ 1u, abort_flag)) ok = false;
                     tcgen05_fence_after_sync();
-                    const uint32_t whole = blocks - (rest != 0 ? 1u : 0u);
+                    uint32_t begun = 0;  // 1: the accumulator holds a part of this piece
                     for (uint32_t kb = 0; ok && kb < whole; ++kb) {
+                        if (LONG && kb != 0 && kb % (kLongBlocks / KPS) == 0) {
+                            // the next piece, in the other accumulator
+                            if (CG == 1) umma_commit(tfull_bar + 8u * (it & 1u)); else umma_commit_pair(tfull_bar + 8u * (it & 1u), 0x3);
+                            ++it;
+                            d_tmem = tmem_base + (it & 1u) * QT;
+                            begun = 0;
+                            if (!mbar_wait(tempty_bar + 8u * (it & 1u), ((it >> 1) & 1u) ^ 1u, abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            tcgen05_fence_after_sync();
+                        }
                         if (!mbar_wait(full_bar + 8u * stage, phase, abort_flag)) {
                             ok = false;
                             break;
@@ -454,9 +538,10 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
 #pragma unroll
                             for (uint32_t k = 0; k < 4; ++k) {
                                 umma_f16<CG>(d_tmem, dp + (P_MN ? 128u : 2u) * k, dq + (WEIGHT ? 128u : 2u) * k, idesc,
-                                             (kb > 0 || j > 0 || k > 0) ? 1u : 0u);
+                                             (j > 0 || k > 0) ? 1u : begun);
                             }
                         }
+                        begun = 1;
                         if (CG == 1) umma_commit(empty_bar + 8u * stage); else umma_commit_pair(empty_bar + 8u * stage, 0x3);
                         if (++stage == STAGES) {
                             stage = 0;
@@ -467,6 +552,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 if constexpr (WEIGHT) {
                     // every lane follows: where the ring stands, and whether to go on
                     ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                    it = __shfl_sync(0xffffffffu, it, 0);
                     if (CG == 2 && cta_rank != 0) {
                         const uint32_t at = stage + blocks - (rest != 0 ? 1u : 0u);
                         stage = at % STAGES;
@@ -512,7 +598,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                                         const uint64_t dp = umma_smem_desc_sw128_mn(slot, 8192u);
                                         const uint64_t dq = umma_smem_desc_sw128_mn(slot + T::kPBytes, 8192u);
                                         for (uint32_t k = 0; k < steps; ++k) {
-                                            umma_f16<CG>(d_tmem, dp + 128u * k, dq + 128u * k, idesc, (blocks > 1u || k > 0) ? 1u : 0u);
+                                            umma_f16<CG>(d_tmem, dp + 128u * k, dq + 128u * k, idesc, (blocks > 1u || k > 0) ? 1u : 0u);  // (joins the last piece)
                                         }
                                         if (CG == 1) umma_commit(empty_bar + 8u * stage); else umma_commit_pair(empty_bar + 8u * stage, 0x3);
                                     }
@@ -530,117 +616,176 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                     }
                 }
                 if (cta_rank == 0 && lane == 0 && ok) {
-                    if (CG == 1) umma_commit(tfull_bar + 8u * acc); else umma_commit_pair(tfull_bar + 8u * acc, 0x3);
+                    if (CG == 1) umma_commit(tfull_bar + 8u * (it & 1u)); else umma_commit_pair(tfull_bar + 8u * (it & 1u), 0x3);
                 }
-                if (!WEIGHT) ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                if (!WEIGHT) {
+                    ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                    it = __shfl_sync(0xffffffffu, it, 0);
+                }
                 ++it;
             }
         }
         __syncwarp();
     } else {
         // ------------------------------------------------------------------ epilogue
-        const uint32_t q = warp & 3u;  // tensor-memory lane quadrant this warp may read
-        uint32_t it = 0, store_buf = 0;
-        for (uint32_t t = worker; t < tiles; t += workers) {
+        // Warp w may read tensor-memory lanes 32 (w % 4) .. + 31; the two warps of a quadrant take alternate chunks of
+        // columns. LONG: the pieces of a tile are added up in `run` as they come; else there is one piece.
+        const uint32_t q = warp & 3u, half = (warp - 2u) >> 2;
+        constexpr uint32_t W = T::kChunk;
+        constexpr uint32_t kChunks = QT / W / 2u;  // of this warp
+        uint8_t *my_ptr = staging_ptr + (warp - 2u) * 4096u;
+        const uint32_t my_staging = staging + (warp - 2u) * 4096u;
+        uint32_t it = 0;
+        bool alive = true;
+        // waits for the accumulator of piece `it`; false: given up
+        auto wait_piece = [&]() -> bool {
+            uint32_t ready = 1;
+            if (lane == 0) ready = mbar_wait(tfull_bar + 8u * (it & 1u), (it >> 1) & 1u, abort_flag) ? 1u : 0u;
+            ready = __shfl_sync(0xffffffffu, ready, 0);
+            tcgen05_fence_after_sync();
+            return ready != 0;
+        };
+        auto release_piece = [&]() {
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 1) mbar_arrive(tempty_bar + 8u * (it & 1u)); else mbar_arrive_cluster(map_to_cta(tempty_bar + 8u * (it & 1u), 0));
+            }
+            ++it;
+        };
+        for (uint32_t t = worker; alive && t < tiles; t += workers) {
             GroupedTile tile;
             if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
             const bool summed = !WEIGHT || tile.valid != 0;  // a group without rows: a gradient of zeros, no accumulator
-            const uint32_t acc = it & 1u;
-            if (summed) {
-                uint32_t ready = 1;
-                if (lane == 0) ready = mbar_wait(tfull_bar + 8u * acc, (it >> 1) & 1u, abort_flag) ? 1u : 0u;
-                ready = __shfl_sync(0xffffffffu, ready, 0);
-                if (!ready) break;
-                tcgen05_fence_after_sync();
-            }
-            const uint32_t taddr = tmem_base + ((q * 32u) << 16) + acc * QT;
             const uint32_t p_warp = tile.p0 + cta_rank * 128u + q * 32u;  // first index on P of this warp's lanes
-            if (!WEIGHT) {
-                const uint32_t col = p_warp + lane;
-                float bias = 0.f;
-                if (FORM == kFormForward && p.bias && col < p.p_dim) {
-                    const size_t at = static_cast<size_t>(tile.group) * p.p_dim + col;
-                    bias = p.in_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[at])
-                                     : __half2float(static_cast<const __half *>(p.bias)[at]);
-                }
-                if (p_warp < p.p_dim) {
-#pragma unroll 1
-                    for (uint32_t c = 0; c * 32u < tile.valid; ++c) {
-                        uint32_t r[32];
-                        tmem_ld_32x32b_x32(taddr + c * 32u, r);
-                        tmem_ld_wait();
-                        if (FORM == kFormForward) {
-                            if (p.bias) {
+            const uint32_t lanes = tmem_base + ((q * 32u) << 16);
+            const uint32_t cols = WEIGHT ? min(static_cast<uint32_t>(QT), p.q_dim - tile.q0) : tile.valid;  // columns stored
+            const bool live = p_warp < p.p_dim && (summed || !p.accumulate);
+            const uint32_t col = p_warp + lane;  // forward, input: this lane's output column
+            float bias = 0.f;
+            if (FORM == kFormForward && p.bias && col < p.p_dim) {
+                const size_t at = static_cast<size_t>(tile.group) * p.p_dim + col;
+                bias = p.in_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[at])
+                                 : __half2float(static_cast<const __half *>(p.bias)[at]);
+            }
+            uint32_t run[LONG ? kChunks * W : 1];
+            if constexpr (LONG) {
+                const uint32_t k_blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks * KPS;
+                // (a tail joins the last piece, so pieces are counted over the whole blocks)
+                const uint32_t whole = WEIGHT ? tile.valid / kStepK : k_blocks;
+                const uint32_t pieces = max((whole + kLongBlocks - 1u) / kLongBlocks, k_blocks != 0 ? 1u : 0u);
 #pragma unroll
-                                for (uint32_t j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + bias);
+                for (uint32_t j = 0; j < kChunks * W; ++j) run[j] = 0u;
+                for (uint32_t piece = 0; alive && piece < pieces; ++piece) {
+                    alive = wait_piece();
+                    if (!alive) break;
+#pragma unroll
+                    for (uint32_t c = 0; c < kChunks * W / 16u; ++c) {
+                        const uint32_t at = (2u * (c * 16u / W) + half) * W + c * 16u % W;
+                        if (at < cols) {
+                            uint32_t r[16];
+                            tmem_ld_32x32b_x16(lanes + (it & 1u) * QT + at, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (uint32_t j = 0; j < 16; ++j) {
+                                run[c * 16u + j] = __float_as_uint(__uint_as_float(run[c * 16u + j]) + __uint_as_float(r[j]));
                             }
-                            if (p.pre) store_transposed32(p.pre, p.out_type, tile.q0 + c * 32u, tile.valid - c * 32u, col, p.p_dim, r, lane);
-                            act_apply<32>(r, p.act);
                         }
-                        store_transposed32(p.out, p.out_type, tile.q0 + c * 32u, tile.valid - c * 32u, col, p.p_dim, r, lane);
+                    }
+                    release_piece();
+                }
+            } else if (summed) {
+                alive = wait_piece();
+            }
+            if (!alive) break;
+            const uint32_t taddr = lanes + (it & 1u) * QT;
+            if (!WEIGHT) {
+                if (live) {
+                    if constexpr (LONG) {
+#pragma unroll
+                        for (uint32_t i = 0; i < kChunks; ++i) {
+                            const uint32_t at = (2u * i + half) * W;
+                            if (at < cols) finish_rows<FORM, W>(p, run + i * W, bias, tile.q0 + at, cols - at, col, lane);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (uint32_t at = half * W; at < cols; at += 2u * W) {
+                            uint32_t r[W];
+                            tmem_ld_columns<W>(taddr + at, r);
+                            tmem_ld_wait();
+                            finish_rows<FORM, W>(p, r, bias, tile.q0 + at, cols - at, col, lane);
+                        }
                     }
                 }
-            } else if (p_warp < p.p_dim && (summed || !p.accumulate)) {
+            } else if (live) {
                 // rows of the result: through swizzled staging (32 rows of 128 bytes) and TMA, which clips what lies
                 // past N and K; with `accumulate` the copy adds to what is there
-                const bool f32 = p.out_type == 2u;
-                uint8_t *my_ptr = staging_ptr + q * 8192u;
-                const uint32_t my_staging = staging + q * 8192u;
-                const uint32_t width = f32 ? 32u : 64u;  // columns of 128 bytes
-                const uint32_t cols = min(static_cast<uint32_t>(QT), p.q_dim - tile.q0);
-#pragma unroll 1
-                for (uint32_t c0 = 0; c0 < cols; c0 += width) {
-                    uint8_t *row_ptr = my_ptr + (store_buf & 1u) * 4096u + lane * 128u;
-                    if (lane == 0) tma_store_wait_read<1>();  // the store issued two chunks ago has read this buffer
+                uint8_t *row_ptr = my_ptr + lane * 128u;
+                auto staging_free = [&]() {
+                    if (lane == 0) tma_store_wait_read<0>();  // the last copy out of it has read it
                     __syncwarp();
-#pragma unroll 1
-                    for (uint32_t part = 0; part * 32u < width; ++part) {
-                        uint32_t r[32];
-                        if (summed) {
-                            tmem_ld_32x32b_x32(taddr + c0 + part * 32u, r);
-                            tmem_ld_wait();
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < 32; ++j) r[j] = 0u;
-                        }
-                        if (f32) {
-#pragma unroll
-                            for (uint32_t j = 0; j < 8; ++j) {
-                                *reinterpret_cast<uint4 *>(row_ptr + ((j ^ (lane & 7u)) << 4)) =
-                                    make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-                            }
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j) {
-                                uint4 v;
-                                v.x = pack2_typed(r[8 * j + 0], r[8 * j + 1], p.out_type);
-                                v.y = pack2_typed(r[8 * j + 2], r[8 * j + 3], p.out_type);
-                                v.z = pack2_typed(r[8 * j + 4], r[8 * j + 5], p.out_type);
-                                v.w = pack2_typed(r[8 * j + 6], r[8 * j + 7], p.out_type);
-                                *reinterpret_cast<uint4 *>(row_ptr + (((part * 4u + j) ^ (lane & 7u)) << 4)) = v;
-                            }
-                        }
-                    }
+                };
+                auto send = [&](uint32_t at) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        const uint32_t src = my_staging + (store_buf & 1u) * 4096u;
-                        const int32_t x = static_cast<int32_t>(tile.q0 + c0), y = static_cast<int32_t>(p_warp);
+                        const int32_t x = static_cast<int32_t>(tile.q0 + at), y = static_cast<int32_t>(p_warp);
                         const int32_t z = static_cast<int32_t>(tile.group);
-                        if (p.accumulate) tma_reduce_add_3d(&p.tm_out, src, x, y, z); else tma_store_3d(&p.tm_out, src, x, y, z);
+                        if (p.accumulate) tma_reduce_add_3d(&p.tm_out, my_staging, x, y, z); else tma_store_3d(&p.tm_out, my_staging, x, y, z);
                         tma_store_commit();
                     }
-                    ++store_buf;
+                };
+                auto put_f32 = [&](const uint32_t *r) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        *reinterpret_cast<uint4 *>(row_ptr + ((j ^ (lane & 7u)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                    }
+                };
+                if constexpr (LONG) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kChunks; ++i) {
+                        const uint32_t at = (2u * i + half) * W;
+                        if (at < cols) {
+                            staging_free();
+                            put_f32(run + i * W);
+                            send(at);
+                        }
+                    }
+                } else {
+                    const bool f32 = p.out_type == 2u;
+                    const uint32_t width = f32 ? 32u : 64u;  // columns of 128 bytes
+#pragma unroll 1
+                    for (uint32_t at = half * width; at < cols; at += 2u * width) {
+                        staging_free();
+#pragma unroll 1
+                        for (uint32_t part = 0; part * 32u < width; ++part) {
+                            uint32_t r[32];
+                            if (summed) {
+                                tmem_ld_32x32b_x32(taddr + at + part * 32u, r);
+                                tmem_ld_wait();
+                            } else {
+#pragma unroll
+                                for (uint32_t j = 0; j < 32; ++j) r[j] = 0u;
+                            }
+                            if (f32) {
+                                put_f32(r);
+                            } else {
+#pragma unroll
+                                for (uint32_t j = 0; j < 4; ++j) {
+                                    uint4 v;
+                                    v.x = pack2_typed(r[8 * j + 0], r[8 * j + 1], p.out_type);
+                                    v.y = pack2_typed(r[8 * j + 2], r[8 * j + 3], p.out_type);
+                                    v.z = pack2_typed(r[8 * j + 4], r[8 * j + 5], p.out_type);
+                                    v.w = pack2_typed(r[8 * j + 6], r[8 * j + 7], p.out_type);
+                                    *reinterpret_cast<uint4 *>(row_ptr + (((part * 4u + j) ^ (lane & 7u)) << 4)) = v;
+                                }
+                            }
+                        }
+                        send(at);
+                    }
                 }
             }
-            if (summed) {
-                tcgen05_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) {
-                    if (CG == 1) mbar_arrive(tempty_bar + 8u * acc); else mbar_arrive_cluster(map_to_cta(tempty_bar + 8u * acc, 0));
-                }
-                ++it;
-            }
+            if (!LONG && summed) release_piece();
         }
         if (WEIGHT && lane == 0) tma_store_wait_read<0>();
         __syncwarp();

@@ -46,10 +46,10 @@ static int launch_attributes(cudaLaunchAttribute *attrs, int cg) {
 
 // `most_tiles`: an upper bound of the tiles there can be; the grid is persistent and never larger than what
 // is resident at once.
-template <int FORM, int CG, int QT, int STAGES, int KPS>
+template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG = false>
 static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uint64_t most_tiles, cudaStream_t stream) {
-    using T = GroupedTraits<FORM, CG, QT, STAGES, KPS>;
-    auto kern = hgemm_grouped_kernel<FORM, CG, QT, STAGES, KPS>;
+    using T = GroupedTraits<FORM, CG, QT, STAGES, KPS, LONG>;
+    auto kern = hgemm_grouped_kernel<FORM, CG, QT, STAGES, KPS, LONG>;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attrs[2];
@@ -90,7 +90,7 @@ static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uin
 template <int FORM>
 static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, size_t p_dim, size_t k_dim, size_t w_rows,
                     size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, cudaStream_t stream) {
-    constexpr int kSlots = FORM == kFormForward ? 96 : 100;
+    constexpr int kSlots = FORM == kFormForward ? 96 : 102;
     p.error_word = st.error_word;
     p.rows = static_cast<uint32_t>(rows);
     p.groups = static_cast<uint32_t>(groups);
@@ -131,12 +131,28 @@ static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, 
     int rc;
     const uint32_t box_rows = FORM == kFormForward ? 128u : 64u;
     if ((rc = get_tensor_map(st, W, w_rows, w_cols, box_rows, 64, &p.tm_p, true, groups, stride_w)) != B200_HGEMM_OK) return rc;
-    for (uint32_t i = 0; i < 4; ++i) {
-        if ((rc = get_tensor_map(st, X, rows, k_dim, 128u >> i, 64, &p.tm_q[i])) != B200_HGEMM_OK) return rc;
+    for (uint32_t i = 0; i < p.q_max / (16u * cg); ++i) {
+        if ((rc = get_tensor_map(st, X, rows, k_dim, 16u * (i + 1u), 64, &p.tm_q[i])) != B200_HGEMM_OK) return rc;
+    }
+    if constexpr (FORM == kFormForward) {
+        if (p.out_type == B200_C_F32 && k_dim > kLongSum) {
+            if (cg == 2) return launch_grouped<FORM, 2, 256, 6, 1, true>(st, kSlots + 3, p, tiles, stream);
+            if (q_cap == 128) return launch_grouped<FORM, 1, 128, 3, 2, true>(st, kSlots + 4, p, tiles, stream);
+            return launch_grouped<FORM, 1, 32, 5, 2, true>(st, kSlots + 5, p, tiles, stream);
+        }
     }
     if (cg == 2) return launch_grouped<FORM, 2, 256, 6, 1>(st, kSlots, p, tiles, stream);
     if (q_cap == 128) return launch_grouped<FORM, 1, 128, 3, 2>(st, kSlots + 1, p, tiles, stream);
     return launch_grouped<FORM, 1, 32, 5, 2>(st, kSlots + 2, p, tiles, stream);
+}
+
+// An operand of the weight form, 64 rows of 64 columns to a box. Where the width is a multiple of 64 the columns are
+// mapped in blocks of 64 and a copy takes two of them; elsewhere such a block would reach into the next row, and
+// past the end of the last one.
+static int columns_map(DeviceState &st, const void *ptr, size_t rows, size_t width, CUtensorMap *map, uint32_t *wide) {
+    *wide = width % 64 == 0 ? 1u : 0u;
+    if (*wide) return get_tensor_map(st, ptr, rows, 64, 64, 64, map, true, width / 64, 64, 2, width, 2);
+    return get_tensor_map(st, ptr, rows, width, 64, 64, map);
 }
 
 // Weight form: dB_g = dZ_g^T A_g.
@@ -162,12 +178,16 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
     const uint64_t tiles = static_cast<uint64_t>(G) * p.p_blocks * p.q_blocks;
     if (tiles > 0x7fffffffull) return B200_HGEMM_ERR_TOO_LARGE;
     int rc;
-    if ((rc = get_tensor_map(st, dZ, M, N, 64, 64, &p.tm_p)) != B200_HGEMM_OK) return rc;
-    if ((rc = get_tensor_map(st, A, M, K, 64, 64, &p.tm_q[0])) != B200_HGEMM_OK) return rc;
+    if ((rc = columns_map(st, dZ, M, N, &p.tm_p, &p.p_wide)) != B200_HGEMM_OK) return rc;
+    if ((rc = columns_map(st, A, M, K, &p.tm_q[0], &p.q_wide)) != B200_HGEMM_OK) return rc;
     const bool f32 = g.db_type == B200_C_F32;
     if ((rc = get_tensor_map(st, dB, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
-    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 104, p, tiles, stream);
-    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 105, p, tiles, stream);
+    if (f32 && M > kLongSum) {
+        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, stream);
+        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, stream);
+    }
+    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 110, p, tiles, stream);
+    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, stream);
 }
 
 // ---- the pass over dC -----------------------------------------------------------------------
@@ -276,6 +296,26 @@ static int check_groups(const int32_t *offsets, size_t N, size_t K, size_t G, si
     return B200_HGEMM_OK;
 }
 
+static GroupedParams forward_params(void *C, const int32_t *offsets, const b200_linear_args &args) {
+    GroupedParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = C;
+    p.pre = args.pre;
+    p.bias = args.bias;
+    p.residual = args.residual;
+    p.offsets = offsets;
+    p.in_bf16 = args.in_type == B200_C_BF16 ? 1u : 0u;
+    p.out_type = static_cast<uint32_t>(args.c_type);
+    p.act = static_cast<uint32_t>(args.act);
+    return p;
+}
+
+int run_linear_rows(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args &args,
+                    cudaStream_t stream) {
+    GroupedParams p = forward_params(C, nullptr, args);
+    return run_rows<kFormForward>(st, A, B, M, N, K, N, K, 1, N * K, p, stream);
+}
+
 static int grouped_forward(const void *A, const void *B, void *C, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
                            size_t stride_b, const b200_linear_args *args, cudaStream_t stream) {
     if (!args || !B || (M > 0 && (!A || !C))) return B200_HGEMM_ERR_INVALID_ARG;
@@ -289,15 +329,7 @@ static int grouped_forward(const void *A, const void *B, void *C, const int32_t 
     DeviceState *st = nullptr;
     if ((rc = current_state(&st)) != B200_HGEMM_OK) return rc;
     if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
-    GroupedParams p;
-    memset(&p, 0, sizeof(p));
-    p.out = C;
-    p.pre = args->pre;
-    p.bias = args->bias;
-    p.offsets = offsets;
-    p.in_bf16 = args->in_type == B200_C_BF16 ? 1u : 0u;
-    p.out_type = static_cast<uint32_t>(args->c_type);
-    p.act = static_cast<uint32_t>(args->act);
+    GroupedParams p = forward_params(C, offsets, *args);
     return run_rows<kFormForward>(*st, A, B, M, N, K, N, K, G, G > 1 ? stride_b : N * K, p, stream);
 }
 

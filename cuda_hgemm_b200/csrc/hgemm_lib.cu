@@ -116,11 +116,13 @@ int current_state(DeviceState **out) {
 // tiles, without. Out-of-range elements read as zero and are dropped on store. The cache is 4-way
 // set-associative (64 sets): a handful of operands in rotation never evict each other.
 int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
-                   CUtensorMap *out, bool swizzle, uint64_t batch, uint64_t batch_stride, uint32_t elem_bytes) {
-    TensorMapKey key{ptr, rows, cols, box_rows, box_cols, swizzle, batch, batch_stride, elem_bytes};
+                   CUtensorMap *out, bool swizzle, uint64_t batch, uint64_t batch_stride, uint32_t elem_bytes,
+                   uint64_t pitch, uint32_t box_batch) {
+    if (pitch == 0) pitch = cols;
+    TensorMapKey key{ptr, rows, cols, box_rows, box_cols, swizzle, batch, batch_stride, elem_bytes, pitch, box_batch};
     size_t h = (reinterpret_cast<uintptr_t>(ptr) >> 8) * 0x9E3779B97F4A7C15ull;
     h ^= rows * 0xC2B2AE3D27D4EB4Full + cols * 0x165667B19E3779F9ull + box_rows * 131u + box_cols + (swizzle ? 0u : 77u) +
-         batch * 0x9E3779B1ull + batch_stride * 0x85EBCA77ull + elem_bytes;
+         batch * 0x9E3779B1ull + batch_stride * 0x85EBCA77ull + elem_bytes + pitch * 0x27D4EB2Full;
     const size_t set = ((h >> 20) & 63u) * kTensorMapWays;
     std::lock_guard<std::mutex> lock(st.mu);
     TensorMapSlot *slot = nullptr;
@@ -139,8 +141,8 @@ int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t col
     // a stack of matrices is a third dimension; a stack of one with stride 0 stays two-dimensional
     const bool stacked = batch > 1 || batch_stride != 0;
     cuuint64_t dims[3] = {cols, rows, batch};
-    cuuint64_t strides[2] = {cols * elem_bytes, (batch_stride ? batch_stride : rows * cols) * elem_bytes};
-    cuuint32_t box[3] = {box_cols, box_rows, 1};
+    cuuint64_t strides[2] = {pitch * elem_bytes, (batch_stride ? batch_stride : rows * cols) * elem_bytes};
+    cuuint32_t box[3] = {box_cols, box_rows, box_batch};
     cuuint32_t elem_strides[3] = {1, 1, 1};
     CUresult r = enc(&slot->map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, stacked ? 3 : 2, const_cast<void *>(ptr), dims, strides, box,
                      elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
@@ -1266,9 +1268,6 @@ static int run_plan(DeviceState &st, const void *A, const void *B, void *C, size
         p.bias = ea.bias;
         p.c_in = ea.c_in;
         p.c_type = ea.c_type;
-        p.act = ea.act;
-        p.pre = ea.pre;
-        p.in_bf16 = ea.in_bf16;
         if (ea.c_type == kOutF32) p.tma_store = 0;  // FP32 rows leave with plain 16-byte stores
     }
 #ifdef B200_TIMELINE
@@ -1831,16 +1830,20 @@ int b200_hgemm_fused_ex(const void *A, const void *B, void *C, size_t M, size_t 
 }
 
 // ---- linear layers --------------------------------------------------------------------------------
-// The dispatch's plan for the shape, as fused_plan gives it. k-ranges summed inside clusters are asked for by name: left
-// to the library they could fall back to a workspace of its own, and this entry point uses the caller's only.
-static int linear_plan(const DeviceState &st, size_t M, size_t N, size_t K, const b200_linear_args &args, b200_hgemm_plan *pl) {
-    const int rc = fused_plan(st, M, N, K, args.c_type, pl);
-    if (rc != B200_HGEMM_OK) return rc;
-    if ((pl->variant == B200_VARIANT_SKINNY || pl->variant == B200_VARIANT_SKINNY_PAIR) && pl->grid == 0 &&
-        skinny_sums_on_chip(*pl, skinny_slices(*pl, st, N, K)) == 1) {
-        pl->grid = 1;
-    }
-    return B200_HGEMM_OK;
+// Whether a linear layer runs on the short-A kernels, with which plan. They take the batches of up to 128 rows that the
+// dispatch gives them; everything else runs on the grouped kernel as a single group (run_linear_rows), whose epilogue
+// keeps up with an activation and with Z beside C: 8192 x 14336 x 4096 in BF16 with gelu and Z takes 903 us there, 1453 us
+// on the whole-tile kernels with their fused epilogue (one row per lane, values one after the other). FP32 results
+// of long sums go there too: see gemm_kernel_grouped.cuh.
+// k-ranges summed inside clusters are asked for by name: left to the library they could fall back to a workspace of
+// its own, and this entry point uses the caller's only.
+static bool linear_plan(const DeviceState &st, size_t M, size_t N, size_t K, const b200_linear_args &args, b200_hgemm_plan *pl) {
+    select_plan(st, M, N, K, pl);
+    if (pl->variant != B200_VARIANT_SKINNY && pl->variant != B200_VARIANT_SKINNY_PAIR) return false;
+    const uint32_t slices = skinny_slices(*pl, st, N, K);
+    if (args.c_type == B200_C_F32 && K > kLongSum * slices) return false;
+    if (pl->grid == 0 && skinny_sums_on_chip(*pl, slices) == 1) pl->grid = 1;
+    return true;
 }
 
 static int check_linear(const void *A, const void *B, const void *C, size_t M, size_t N, size_t K, const b200_linear_args *args) {
@@ -1850,7 +1853,9 @@ static int check_linear(const void *A, const void *B, const void *C, size_t M, s
     if (args->in_type != B200_C_F16 && args->in_type != B200_C_BF16) return B200_HGEMM_ERR_INVALID_ARG;
     if (args->c_type != args->in_type && args->c_type != B200_C_F32) return B200_HGEMM_ERR_INVALID_ARG;
     if (K % 8 != 0) return B200_HGEMM_ERR_UNSUPPORTED;
-    return B200_HGEMM_OK;
+    uintptr_t bits = 0;
+    for (const void *ptr : {A, B, C, args->bias, args->residual, static_cast<const void *>(args->pre)}) bits |= reinterpret_cast<uintptr_t>(ptr);
+    return (bits & 15u) ? B200_HGEMM_ERR_MISALIGNED : B200_HGEMM_OK;
 }
 
 size_t b200_hgemm_linear_workspace_bytes(size_t M, size_t N, size_t K, const b200_linear_args *args) {
@@ -1863,8 +1868,7 @@ size_t b200_hgemm_linear_workspace_bytes(size_t M, size_t N, size_t K, const b20
         st = &nominal;
     }
     b200_hgemm_plan pl;
-    if (linear_plan(*st, M, N, K, *args, &pl) != B200_HGEMM_OK) return 0;
-    return b200_hgemm_workspace_bytes(M, N, K, &pl);
+    return linear_plan(*st, M, N, K, *args, &pl) ? b200_hgemm_workspace_bytes(M, N, K, &pl) : 0;
 }
 
 int b200_hgemm_linear(const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args *args,
@@ -1877,8 +1881,7 @@ int b200_hgemm_linear(const void *A, const void *B, void *C, size_t M, size_t N,
     if (rc != B200_HGEMM_OK) return rc;
     if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
     b200_hgemm_plan pl;
-    rc = linear_plan(*st, M, N, K, *args, &pl);
-    if (rc != B200_HGEMM_OK) return rc;
+    if (!linear_plan(*st, M, N, K, *args, &pl)) return run_linear_rows(*st, A, B, C, M, N, K, *args, reinterpret_cast<cudaStream_t>(stream));
     const size_t need = b200_hgemm_workspace_bytes(M, N, K, &pl);
     if (need > 0) {
         if (!workspace || workspace_bytes < need) return B200_HGEMM_ERR_WORKSPACE;

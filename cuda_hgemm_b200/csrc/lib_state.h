@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/b200_hgemm.h"
+
 #include <atomic>
 #include <mutex>
 #include <vector>
@@ -21,9 +23,12 @@ struct TensorMapKey {
     bool swizzle;
     uint64_t batch, batch_stride;  // stacks of matrices: how many, and elements from one to the next (1, 0: a single matrix)
     uint32_t elem_bytes;           // 2: 16-bit elements of either kind (a copy does not tell them apart), 4: FP32
+    uint64_t pitch;                // elements from row to row
+    uint32_t box_batch;            // matrices a box spans
     bool operator==(const TensorMapKey &o) const {
         return ptr == o.ptr && rows == o.rows && cols == o.cols && box_rows == o.box_rows && box_cols == o.box_cols &&
-               swizzle == o.swizzle && batch == o.batch && batch_stride == o.batch_stride && elem_bytes == o.elem_bytes;
+               swizzle == o.swizzle && batch == o.batch && batch_stride == o.batch_stride && elem_bytes == o.elem_bytes &&
+               pitch == o.pitch && box_batch == o.box_batch;
     }
 };
 
@@ -75,8 +80,15 @@ bool cuda_ok(cudaError_t e, const char *what);
 int current_state(DeviceState **out);
 // The tensor map of a row-major matrix (or stack of matrices) viewed through boxes, from the cache or encoded.
 int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
-                   CUtensorMap *out, bool swizzle = true, uint64_t batch = 1, uint64_t batch_stride = 0, uint32_t elem_bytes = 2);
+                   CUtensorMap *out, bool swizzle = true, uint64_t batch = 1, uint64_t batch_stride = 0, uint32_t elem_bytes = 2,
+                   uint64_t pitch = 0, uint32_t box_batch = 1);
 bool pdl_enabled();
+
+// Longest sum an FP32 result may take from one accumulator of the tensor cores (gemm_kernel_grouped.cuh says why).
+constexpr uint32_t kLongSum = 1024;
+// A linear layer on the grouped kernel, all rows one group (arguments checked by the caller).
+int run_linear_rows(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args &args,
+                    cudaStream_t stream);
 
 inline uint32_t ceil_div_u32(uint64_t a, uint64_t b) {
     return static_cast<uint32_t>((a + b - 1) / b);

@@ -183,6 +183,33 @@ def test_linear_forward_large_tiles(cuda_device, dtype, act, with_pre):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_fp32_results_of_long_sums(cuda_device, dtype):
+    """The tensor cores cut an accumulator off at every MMA, on average by half of 2^-23 of it: a sum of 1024 (64 MMAs)
+    is off by at most 64 * 2^-24 in the mean, and so is a longer one, whose pieces are added in FP32 (rounding to
+    nearest adds 2^-24 each, at random). One accumulator for all of a sum of 16384 would be off by sixteen times that."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    limit = 64 * 2.0 ** -24 + 16 * 2.0 ** -24 / 4
+    for M, N, K in ((16, 264, 16384), (200, 264, 16384), (2000, 2568, 16384)):
+        A, B = make((M, K), dtype, cuda_device, 1), make((N, K), dtype, cuda_device, 2)
+        C = torch.empty((M, N), device=cuda_device)
+        api.hgemm_linear(A, B, C)
+        ref = A.double() @ B.double().T
+        assert ((C.double() - ref).norm() / ref.norm()).item() < limit, (M, N, K)
+    for M, N, K in ((16384, 72, 136), (16384, 2568, 2056)):
+        A, dC = make((M, K), dtype, cuda_device, 1), make((M, N), dtype, cuda_device, 2)
+        B = torch.zeros((N, K), dtype=A.dtype, device=cuda_device)
+        dB = torch.empty((N, K), device=cuda_device)
+        api.hgemm_linear_backward(dC, A, B, dB=dB)
+        ref = dC.double().T @ A.double()
+        assert ((dB.double() - ref).norm() / ref.norm()).item() < limit, (M, N, K)
+    assert api.last_device_error() == 0
+
+
+@pytest.mark.gpu
 def test_linear_residual_in_place_and_no_rows(cuda_device):
     import torch
 
@@ -333,6 +360,8 @@ def test_grouped_forward_on_pairs(cuda_device, dtype, out, act):
     """Enough tiles for the pair kernel: several blocks of rows per group, a stack with gaps, a ragged last block."""
     sizes = [400, 37, 0, 1031, 256, 300, 511, 222]
     forward_of_groups(cuda_device, sizes, 1416, 328, dtype, out, act, True, act != "none", gap=8)
+    if out == F32:  # a long sum, added up in pieces
+        forward_of_groups(cuda_device, sizes, 1416, 2184, dtype, out, act, True, False)
 
 
 def backward_of_groups(device, sizes, N, K, dtype, out, act, db_type, gap=0, accumulate=False):
@@ -377,7 +406,7 @@ def test_grouped_backward(cuda_device, sizes, shape):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(1416, 328), (328, 1416), (1032, 776), (2048, 1024)], ids=str)
+@pytest.mark.parametrize("shape", [(1416, 328), (328, 1416), (1032, 776), (2048, 1024), (1344, 1088)], ids=str)
 @pytest.mark.parametrize("dtype,db_type", [(F16, F16), (BF16, F32)])
 def test_grouped_backward_on_pairs(cuda_device, shape, dtype, db_type):
     N, K = shape
