@@ -10,6 +10,7 @@ torch is used for device memory and streams only; the arithmetic is the native l
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 from . import _native
@@ -55,7 +56,7 @@ def _shape_of(A, B, C, c_dtypes=None):
 def _stream_of(t) -> int:
     import torch
 
-    return int(torch.cuda.current_stream(t.device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())  # (the public call builds a Stream object: 3 us of a call's 17)
 
 
 def _call(symbol: str, A, B, C):
@@ -186,7 +187,7 @@ ACTIVATIONS = {"none": _native.ACT_NONE, "relu": _native.ACT_RELU, "gelu": _nati
 def _type_code(dtype):
     import torch
 
-    return {torch.float16: _native.C_F16, torch.bfloat16: _native.C_BF16, torch.float32: _native.C_F32}.get(dtype)
+    return _native.C_F16 if dtype is torch.float16 else _native.C_BF16 if dtype is torch.bfloat16 else _native.C_F32 if dtype is torch.float32 else None
 
 
 def _act_code(act):
@@ -197,17 +198,16 @@ def _act_code(act):
 
 
 def _operand(name, t, dtypes, shape, device):
-    """A contiguous CUDA tensor of one of ``dtypes`` and of ``shape``; its address (``None`` for an absent one)."""
-    import torch
-
+    """A contiguous CUDA tensor of one of ``dtypes`` and of ``shape`` on device number ``device``; its address (``None`` for an
+    absent one)."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or not t.is_cuda or not t.is_contiguous():
+    if getattr(t, "dtype", None) not in dtypes or not t.is_cuda or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous CUDA tensor of type {' or '.join(str(d)[6:] for d in dtypes)}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} must live on {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must live on cuda:{device}")
     return t.data_ptr()
 
 
@@ -217,13 +217,13 @@ def _rows_and_weights(A, B, offsets):
 
     grouped = offsets is not None
     for name, t, dims in (("A", A, 2), ("B", B, 3 if grouped else 2)):
-        if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float16, torch.bfloat16) or not t.is_cuda:
+        if getattr(t, "dtype", None) not in (torch.float16, torch.bfloat16) or not t.is_cuda:
             raise TypeError(f"{name} must be a float16 or bfloat16 CUDA tensor")
         if t.dim() != dims:
             raise ValueError(f"{name} must be {dims}-D")
     if A.dtype != B.dtype:
         raise TypeError("A and B must have one type")
-    if A.device != B.device:
+    if A.get_device() != B.get_device():
         raise ValueError("A and B must live on one device")
     M, K = A.shape
     N = B.shape[-2]
@@ -239,13 +239,23 @@ def _rows_and_weights(A, B, offsets):
     # the matrices must be dense (a dimension of one element may have any stride); the stack may have gaps
     if (B.stride(2) != 1 and K > 1) or (B.stride(1) != K and N > 1):
         raise ValueError("the matrices of B must be contiguous")
-    if not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int32 or not offsets.is_cuda or not offsets.is_contiguous():
+    if getattr(offsets, "dtype", None) != torch.int32 or not offsets.is_cuda or not offsets.is_contiguous():
         raise TypeError("offsets must be a contiguous int32 CUDA tensor")
-    if tuple(offsets.shape) != (G + 1,):
+    if offsets.shape != (G + 1,):
         raise ValueError(f"offsets must have {G + 1} values, one more than B has matrices")
-    if offsets.device != A.device:
+    if offsets.get_device() != A.get_device():
         raise ValueError("offsets must live on A's device")
     return M, N, K, G, B.stride(0) if G > 1 else N * K
+
+
+_NOTHING = contextlib.nullcontext()
+
+
+def _on_device(t):
+    """A context in which ``t``'s device is the current one (nothing to do where it is already)."""
+    import torch
+
+    return _NOTHING if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
 
 
 def _scratch(nbytes, device):
@@ -258,13 +268,13 @@ def _scratch(nbytes, device):
 def _linear_args(A, C, bias, act, residual, pre, bias_shape, M, N):
     import torch
 
-    types = (A.dtype, torch.float32)
-    c_ptr = _operand("C", C, types, (M, N), A.device)
+    dtype, device = A.dtype, A.get_device()
+    c_ptr = _operand("C", C, (dtype, torch.float32), (M, N), device)
     if c_ptr is None:
         raise TypeError("C must be a CUDA tensor")
     return c_ptr, _native.LinearArgs(
-        _type_code(A.dtype), _type_code(C.dtype), _act_code(act), _operand("bias", bias, (A.dtype,), bias_shape, A.device),
-        _operand("residual", residual, (C.dtype,), (M, N), A.device), _operand("pre", pre, (C.dtype,), (M, N), A.device))
+        _type_code(dtype), _type_code(C.dtype), _act_code(act), _operand("bias", bias, (dtype,), bias_shape, device),
+        _operand("residual", residual, (C.dtype,), (M, N), device), _operand("pre", pre, (C.dtype,), (M, N), device))
 
 
 def hgemm_linear(A, B, C, bias=None, act: str = "none", residual=None, pre=None):
@@ -273,16 +283,17 @@ def hgemm_linear(A, B, C, bias=None, act: str = "none", residual=None, pre=None)
     ``A [M, K]``, ``B [N, K]`` and ``bias [N]`` are float16 or bfloat16 (all of one type), ``C``, ``residual`` and ``pre``
     ``[M, N]`` of that type or float32. ``act`` is one of ``ACTIVATIONS``. ``pre`` receives ``A @ B.T + bias``, which
     :func:`hgemm_linear_backward` needs; ``residual`` may be ``C`` itself. ``K`` is a multiple of 8; ``M`` may be 0."""
-    import torch
-
     M, N, K, _, _ = _rows_and_weights(A, B, None)
     c_ptr, args = _linear_args(A, C, bias, act, residual, pre, (N,), M, N)
-    lib = _native.load()
-    with torch.cuda.device(A.device):
-        nbytes = lib.b200_hgemm_linear_workspace_bytes(M, N, K, ctypes.byref(args))
-        ws = _scratch(nbytes, A.device)
-        check(lib.b200_hgemm_linear(A.data_ptr(), B.data_ptr(), c_ptr, M, N, K, ctypes.byref(args),
-                                    ws.data_ptr() if ws is not None else None, nbytes, _stream_of(A)))
+    lib, ref = _native.load(), ctypes.byref(args)
+    with _on_device(A):
+        stream = _stream_of(A)
+        status = lib.b200_hgemm_linear(A.data_ptr(), B.data_ptr(), c_ptr, M, N, K, ref, None, 0, stream)
+        if status == _native.ERR_WORKSPACE:  # few shapes need any (k cut into more ranges than a cluster holds)
+            nbytes = lib.b200_hgemm_linear_workspace_bytes(M, N, K, ref)
+            ws = _scratch(nbytes, A.device)
+            status = lib.b200_hgemm_linear(A.data_ptr(), B.data_ptr(), c_ptr, M, N, K, ref, ws.data_ptr(), nbytes, stream)
+        check(status)
     return C
 
 
@@ -294,13 +305,11 @@ def hgemm_grouped(A, B, C, offsets, bias=None, act: str = "none", pre=None):
     ``bias [G, N]`` are float16 or bfloat16, ``C`` and ``pre`` ``[M, N]`` of that type or float32. ``offsets`` are ``G + 1``
     ascending int32 values on the device, read there by the kernel: the host never needs the group sizes. Groups may
     be empty; rows outside ``offsets[0] : offsets[G]`` are not written. ``K`` is a multiple of 8, ``G`` at most 1024."""
-    import torch
-
     if offsets is None:
         raise TypeError("offsets must be a contiguous int32 CUDA tensor")
     M, N, K, G, stride = _rows_and_weights(A, B, offsets)
     c_ptr, args = _linear_args(A, C, bias, act, None, pre, (G, N), M, N)
-    with torch.cuda.device(A.device):
+    with _on_device(A):
         check(_native.load().b200_hgemm_grouped(A.data_ptr(), B.data_ptr(), c_ptr, offsets.data_ptr(), M, N, K, G, stride,
                                                 ctypes.byref(args), _stream_of(A)))
     return C
@@ -310,8 +319,8 @@ def _backward(dC, A, B, offsets, act, pre, dA, dB, dbias, dZ, accumulate):
     import torch
 
     M, N, K, G, stride = _rows_and_weights(A, B, offsets)
-    dtype, device = A.dtype, A.device
-    if not isinstance(dC, torch.Tensor):
+    dtype, device = A.dtype, A.get_device()
+    if dC is None:
         raise TypeError("dC must be a CUDA tensor")
     dc_ptr = _operand("dC", dC, (dtype, torch.float32), (M, N), device)
     stack = (G,) if offsets is not None else ()
@@ -321,15 +330,15 @@ def _backward(dC, A, B, offsets, act, pre, dA, dB, dbias, dZ, accumulate):
     if dA is None and dB is None and dbias is None and dZ is None:
         raise ValueError("none of dA, dB, dbias and dZ was asked for")
     grads = _native.LinearGrads(
-        _type_code(dtype), _type_code(dC.dtype), code, _type_code(dB.dtype) if isinstance(dB, torch.Tensor) else _type_code(dtype),
+        _type_code(dtype), _type_code(dC.dtype), code, _type_code(dtype if dB is None else getattr(dB, "dtype", None)) or 0,
         1 if accumulate else 0, dc_ptr, _operand("pre", pre, (dC.dtype,), (M, N), device),
         _operand("dZ", dZ, (dtype,), (M, N), device), _operand("dA", dA, (dtype,), (M, K), device),
         _operand("dB", dB, (dtype, torch.float32), stack + (N, K), device),
         _operand("dbias", dbias, (torch.float32,), stack + (N,), device))
     lib = _native.load()
-    with torch.cuda.device(device):
+    with _on_device(A):
         nbytes = lib.b200_hgemm_backward_workspace_bytes(M, N, K, G, ctypes.byref(grads))
-        ws = _scratch(nbytes, device)
+        ws = _scratch(nbytes, A.device)
         ws_ptr = ws.data_ptr() if ws is not None else None
         if offsets is None:
             check(lib.b200_hgemm_linear_backward(A.data_ptr(), B.data_ptr(), M, N, K, ctypes.byref(grads), ws_ptr, nbytes,

@@ -257,10 +257,14 @@ struct EpilogueArgs {
     uint32_t in_bf16;  // A, B and bias are BF16
 };
 
+__device__ __forceinline__ float load_bias(const __half *bias, uint32_t col, uint32_t bf16) {
+    return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(bias)[col]) : __half2float(bias[col]);
+}
+
 // v = act(alpha * v + bias[col]) + beta * c_in[row][col] for one element (callers check the bounds).
 __device__ __forceinline__ float fused_value(const EpilogueArgs &e, float acc, size_t row, uint32_t col, uint32_t n) {
     float v = e.alpha * acc;
-    if (e.bias) v += e.in_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(e.bias)[col]) : __half2float(e.bias[col]);
+    if (e.bias) v += load_bias(e.bias, col, e.in_bf16);
     if (e.pre) store_c_elem(e.pre, row * n + col, v, e.c_type);
     if (e.act != kActNone) {
         uint32_t bits = __float_as_uint(v);

@@ -268,16 +268,23 @@ template <int COUNT>
 __device__ __forceinline__ void add_residual(const void *residual, uint32_t type, uint32_t q0, uint32_t valid, uint32_t col,
                                              uint32_t dim, uint32_t *r) {
     const size_t at = static_cast<size_t>(q0) * dim + col;
+    float v[COUNT];
+    // (one loop per type: a choice between them inside would be a branch between every two loads, and the loads
+    // would come back one at a time -- 28 us at 777 x 4099)
+    if (type == 2u) {
 #pragma unroll
-    for (uint32_t j = 0; j < COUNT; ++j) {
-        if (j < valid && col < dim) {
-            const size_t i = at + static_cast<size_t>(j) * dim;
-            const float v = type == 2u ? static_cast<const float *>(residual)[i]
-                            : type == 1u ? __bfloat162float(static_cast<const __nv_bfloat16 *>(residual)[i])
-                                         : __half2float(static_cast<const __half *>(residual)[i]);
-            r[j] = __float_as_uint(__uint_as_float(r[j]) + v);
+        for (uint32_t j = 0; j < COUNT; ++j) v[j] = j < valid && col < dim ? static_cast<const float *>(residual)[at + static_cast<size_t>(j) * dim] : 0.f;
+    } else {
+        unsigned short bits[COUNT];
+#pragma unroll
+        for (uint32_t j = 0; j < COUNT; ++j) {
+            bits[j] = j < valid && col < dim ? static_cast<const unsigned short *>(residual)[at + static_cast<size_t>(j) * dim] : static_cast<unsigned short>(0);
         }
+#pragma unroll
+        for (uint32_t j = 0; j < COUNT; ++j) v[j] = type == 1u ? __uint_as_float(static_cast<uint32_t>(bits[j]) << 16) : __half2float(__ushort_as_half(bits[j]));
     }
+#pragma unroll
+    for (uint32_t j = 0; j < COUNT; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + v[j]);
 }
 
 // What becomes of COUNT columns of an accumulator of the forward or input form.
@@ -667,6 +674,15 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 const size_t at = static_cast<size_t>(tile.group) * p.p_dim + col;
                 bias = p.in_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[at])
                                  : __half2float(static_cast<const __half *>(p.bias)[at]);
+            }
+            if (FORM == kFormForward && p.residual && live) {
+                // the residual's rows of this warp, into L2 while the sums run: one row of a chunk per lane.
+                const size_t size = p.out_type == 2u ? 4u : 2u;
+                for (uint32_t at = half * W + lane; at < cols && lane < W; at += 2u * W) {
+                    const uint8_t *row = static_cast<const uint8_t *>(p.residual) + (static_cast<size_t>(tile.q0 + at) * p.p_dim + p_warp) * size;
+                    prefetch_l2(row);
+                    if (size == 4u) prefetch_l2(row + min(124u, (p.p_dim - p_warp - 1u) * 4u));  // 128 bytes may lie in two lines
+                }
             }
             uint32_t run[LONG ? kChunks * W : 1];
             if constexpr (LONG) {

@@ -80,6 +80,43 @@ struct SkinnyTraits {
     static_assert(STAGES * kStageBytes >= MT * 128 * 2, "the ring must hold one tile of C for the epilogue");
 };
 
+// The epilogue on 16 rows of one column of C, in place (FP32 bit patterns): rows row0 ... row0 + 15, of which those
+// below e's M exist. The same arithmetic as fused_value; the bias was read while the sums were still running, the
+// choice of the activation is made once, and the 16 values of c_in are asked for together.
+__device__ __forceinline__ void fused_rows16(const EpilogueArgs &e, uint32_t (&r)[16], float bias, uint32_t row0, uint32_t m,
+                                             uint32_t col, uint32_t n) {
+    const size_t at = static_cast<size_t>(row0) * n + col;
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) {
+        float v = e.alpha * __uint_as_float(r[j]);
+        if (e.bias) v += bias;
+        r[j] = __float_as_uint(v);
+    }
+    if (e.pre) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            if (row0 + j < m) store_c_elem(e.pre, at + static_cast<size_t>(j) * n, __uint_as_float(r[j]), e.c_type);
+        }
+    }
+    act_apply<16>(r, e.act);
+    if (e.beta != 0.f && e.c_in) {
+        float c[16];
+        // one loop per type, or the loads would come back one at a time
+        if (e.c_type == kOutF32) {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) c[j] = row0 + j < m ? load_c_elem(e.c_in, at + static_cast<size_t>(j) * n, kOutF32) : 0.f;
+        } else if (e.c_type == kOutBF16) {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) c[j] = row0 + j < m ? load_c_elem(e.c_in, at + static_cast<size_t>(j) * n, kOutBF16) : 0.f;
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) c[j] = row0 + j < m ? load_c_elem(e.c_in, at + static_cast<size_t>(j) * n, kOutF16) : 0.f;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) r[j] = __float_as_uint(fmaf(e.beta, c[j], __uint_as_float(r[j])));
+    }
+}
+
 // EPI: whole results get alpha * acc + beta * c_in + bias before their one rounding and leave in epi.c_type
 // (FP32 partials of cut k-ranges are left as they are: skinny_reduce_kernel applies the same to their sum).
 //
@@ -269,6 +306,15 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
         const bool col_live = n < p.n && col_in_tile < p.tile_w;
         const bool staged = p.slices == 1 && p.tma_store != 0;  // whole results, through shared memory and one TMA store
         pdl_wait_prior_grids();  // C (or the workspace) may still be read by the previous kernel
+        float bias = 0.f;
+        if (EPI && !CK && col_live && p.epi.bias) bias = load_bias(p.epi.bias, n, p.epi.in_bf16);
+        if (EPI && !CK && p.slices == 1 && p.epi.beta != 0.f && p.epi.c_in && n0 + q * 32u < p.n) {
+            // c_in's part of this warp, into L2 meanwhile: one row of the tile per lane
+            const size_t size = p.epi.c_type == kOutF32 ? 4u : 2u;
+            for (uint32_t m = lane; m < p.m; m += 32u) {
+                prefetch_l2(static_cast<const uint8_t *>(p.epi.c_in) + (static_cast<size_t>(m) * p.n + n0 + q * 32u) * size);
+            }
+        }
         if (lane == 0) ready = mbar_wait(tfull_bar, 0, abort_flag) ? 1u : 0u;
         ready = __shfl_sync(0xffffffffu, ready, 0);
         if (ready && !CK) {
@@ -283,15 +329,15 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
                 uint32_t r[16];
                 tmem_ld_32x32b_x16(taddr + c * 16u, r);
                 tmem_ld_wait();
+                if (EPI && p.slices == 1 && col_live) fused_rows16(p.epi, r, bias, c * 16u, p.m, n, p.n);
                 if (staged) {
                     if (col_in_tile < p.tile_w) {
 #pragma unroll
                         for (uint32_t j = 0; j < 16; ++j) {
                             // 32 lanes write 32 consecutive halves of one row of the tile
                             const uint32_t m = c * 16u + j;
-                            float v = __uint_as_float(r[j]);
+                            const float v = __uint_as_float(r[j]);
                             if (EPI) {
-                                if (m < p.m && n < p.n) v = fused_value(p.epi, v, m, n, p.n);
                                 store_c_elem(tile_c, m * p.tile_w + col_in_tile, v, p.epi.c_type);  // FP16 or BF16 here
                             } else {
                                 tile_c[m * p.tile_w + col_in_tile] = __float2half_rn(v);
@@ -306,8 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
                             // 32 lanes write 32 consecutive elements of one row of C
                             if (m < p.m) {
                                 if (EPI) {
-                                    store_c_elem(p.c, static_cast<size_t>(m) * p.n + n,
-                                                 fused_value(p.epi, __uint_as_float(r[j]), m, n, p.n), p.epi.c_type);
+                                    store_c_elem(p.c, static_cast<size_t>(m) * p.n + n, __uint_as_float(r[j]), p.epi.c_type);
                                 } else {
                                     p.c[static_cast<size_t>(m) * p.n + n] = __float2half_rn(__uint_as_float(r[j]));
                                 }

@@ -1,5 +1,6 @@
 // Host side of the feed-forward products (include/b200_hgemm.h): argument checks, the choice of tile and the
 // launches of the grouped kernel in its three forms and of the pass over an output's gradient.
+#include <math.h>
 #include <string.h>
 
 #include "../../include/b200_hgemm.h"
@@ -86,47 +87,76 @@ static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uin
     return B200_HGEMM_OK;
 }
 
+// The kernels of the forward and input form: CTAs per tile, most rows of a tile, k-blocks per stage.
+enum RowsKernel : uint32_t { kRowsPair256, kRowsPair128, kRowsSingle128, kRowsSingle32 };
+struct RowsKernelShape {
+    int cg;
+    uint32_t q_cap;
+    int kps;
+};
+constexpr RowsKernelShape rows_kernels[4] = {{2, 256, 1}, {2, 128, 2}, {1, 128, 2}, {1, 32, 2}};
+
+struct RowsPlan {
+    uint32_t kernel;
+    uint32_t q_max;
+};
+
+// The kernel and the most rows per block that should take the least time: waves of tiles times the time of one.
+// A k-block of a tile takes the longest of what the issuing thread needs (0.28 us with one k-block to a stage, 0.20
+// with two), the MMAs (0.27 us for 128 x 256 outputs per CTA) and the operands' way from L2 (11.5 TB/s for all
+// SMs together: what tiles of few rows run into); the start costs about 3 us, 1.2 more where two CTAs have to meet, and
+// the last epilogue 12 ns a row. Group sizes are not known here: the estimate spreads the rows evenly over the groups. Measured
+// over 25 shapes with every kernel and height forced, the choice was the fastest or within 5 percent of it in all but
+// three (10 percent); e.g. 777 x 4099 x 2056: pairs with blocks of 224 rows 24.6 us, single CTAs 33.5; 512 x 4096 x
+// 14336: pairs with 128 rows 58.8, with 256 rows 75.7; 200 x 1024 x 1024: single CTAs 8.1, pairs 9.8.
+static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_dim, size_t k_dim, size_t groups) {
+    const uint64_t live = groups < rows ? groups : rows;  // groups that can hold any rows
+    const uint64_t average = (rows + live - 1) / live;
+    RowsPlan best{kRowsSingle32, 32};
+    if (average <= 32) return best;
+    double best_us = 1e30;
+    for (uint32_t kernel = kRowsPair256; kernel <= kRowsSingle128; ++kernel) {
+        const RowsKernelShape &shape = rows_kernels[kernel];
+        const double slots = st.sm_count / shape.cg;
+        for (uint32_t q_max = shape.q_cap; q_max >= 32u; q_max -= 32u) {
+            if (kernel == kRowsPair256 && q_max < 160u) break;  // the other pair kernel's
+            const uint64_t blocks = (average + q_max - 1) / q_max;
+            const double q = static_cast<double>((average + blocks - 1) / blocks);
+            const double tiles = static_cast<double>(blocks * live) * ceil_div_u32(p_dim, 128u * shape.cg);
+            const double active = tiles < slots ? tiles : slots;
+            const double operands = active * shape.cg * (16384.0 + q / shape.cg * 128.0);
+            double per_block = operands / 11.5e6;
+            const double mma = 0.27 * q / 256.0, issue = shape.kps == 2 ? 0.20 : 0.28;
+            if (per_block < mma) per_block = mma;
+            if (per_block < issue) per_block = issue;
+            const double waves = ceil(tiles / slots);
+            const double us = waves * per_block * ceil_div_u32(k_dim, 64) + (shape.cg == 2 ? 4.2 : 3.0) + 0.012 * q;
+            if (us < best_us * 0.999) {
+                best_us = us;
+                best = RowsPlan{kernel, q_max};
+            }
+        }
+    }
+    return best;
+}
+
 // Forward and input form. X: the rows' operand [rows x k_dim]; W: groups matrices [w_rows x w_cols], stride_w apart.
 template <int FORM>
 static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, size_t p_dim, size_t k_dim, size_t w_rows,
                     size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, cudaStream_t stream) {
-    constexpr int kSlots = FORM == kFormForward ? 96 : 102;
+    constexpr int kSlots = FORM == kFormForward ? 96 : 104;
     p.error_word = st.error_word;
     p.rows = static_cast<uint32_t>(rows);
     p.groups = static_cast<uint32_t>(groups);
     p.p_dim = static_cast<uint32_t>(p_dim);
-    // Tile: pairs on 256 x 256 once they fill the GPU; single CTAs on 128 columns of weights and up to 128 rows
-    // below that, with blocks of rows halved until every SM has a tile; and where the groups hold no more than 32 rows
-    // on average, a ring of weights with little room for rows (decode: bound by reading the weights once).
-    const uint64_t average = (rows + groups - 1) / groups;
-    const uint64_t sms = static_cast<uint64_t>(st.sm_count);
-    auto most_tiles = [&](uint64_t width, uint64_t q_max) {
-        const uint64_t blocks = rows / q_max + (groups < rows ? groups : rows);
-        return blocks * ceil_div_u32(p_dim, width);
-    };
-    auto few_tiles = [&](uint64_t width, uint64_t q_max) {
-        const uint64_t blocks = (average + q_max - 1) / q_max * (groups < rows ? groups : rows);
-        return blocks * ceil_div_u32(p_dim, width);
-    };
-    int cg = 1, kps = 2;
-    uint32_t q_cap = 32;
-    p.q_max = 32;
-    if (average > 32) {
-        if (few_tiles(256, 256) >= sms / 2) {
-            cg = 2;
-            kps = 1;
-            q_cap = 256;
-            p.q_max = 256;
-        } else {
-            q_cap = 128;
-            p.q_max = 128;
-            while (p.q_max > 32 && few_tiles(128, p.q_max) < sms) p.q_max /= 2;
-        }
-    }
+    const RowsPlan plan = choose_rows_plan(st, rows, p_dim, k_dim, groups);
+    const int cg = rows_kernels[plan.kernel].cg, kps = rows_kernels[plan.kernel].kps;
+    p.q_max = plan.q_max;
     p.p_blocks = ceil_div_u32(p_dim, 128u * cg);
     p.p_div = make_fast_div(p.p_blocks);
     p.k_blocks = ceil_div_u32(k_dim, 64u * kps);
-    const uint64_t tiles = most_tiles(128u * cg, p.q_max);
+    // an upper bound: every group may end in a block that is not full
+    const uint64_t tiles = (rows / p.q_max + (groups < rows ? groups : rows)) * p.p_blocks;
     if (tiles > 0x7fffffffull) return B200_HGEMM_ERR_TOO_LARGE;
     int rc;
     const uint32_t box_rows = FORM == kFormForward ? 128u : 64u;
@@ -134,16 +164,23 @@ static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, 
     for (uint32_t i = 0; i < p.q_max / (16u * cg); ++i) {
         if ((rc = get_tensor_map(st, X, rows, k_dim, 16u * (i + 1u), 64, &p.tm_q[i])) != B200_HGEMM_OK) return rc;
     }
+    const int slot = kSlots + static_cast<int>(plan.kernel);
     if constexpr (FORM == kFormForward) {
         if (p.out_type == B200_C_F32 && k_dim > kLongSum) {
-            if (cg == 2) return launch_grouped<FORM, 2, 256, 6, 1, true>(st, kSlots + 3, p, tiles, stream);
-            if (q_cap == 128) return launch_grouped<FORM, 1, 128, 3, 2, true>(st, kSlots + 4, p, tiles, stream);
-            return launch_grouped<FORM, 1, 32, 5, 2, true>(st, kSlots + 5, p, tiles, stream);
+            switch (plan.kernel) {
+                case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, stream);
+                case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, stream);
+                case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, stream);
+                default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, stream);
+            }
         }
     }
-    if (cg == 2) return launch_grouped<FORM, 2, 256, 6, 1>(st, kSlots, p, tiles, stream);
-    if (q_cap == 128) return launch_grouped<FORM, 1, 128, 3, 2>(st, kSlots + 1, p, tiles, stream);
-    return launch_grouped<FORM, 1, 32, 5, 2>(st, kSlots + 2, p, tiles, stream);
+    switch (plan.kernel) {
+        case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1>(st, slot, p, tiles, stream);
+        case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2>(st, slot, p, tiles, stream);
+        case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2>(st, slot, p, tiles, stream);
+        default: return launch_grouped<FORM, 1, 32, 5, 2>(st, slot, p, tiles, stream);
+    }
 }
 
 // An operand of the weight form, 64 rows of 64 columns to a box. Where the width is a multiple of 64 the columns are
@@ -193,7 +230,13 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
 // ---- the pass over dC -----------------------------------------------------------------------
 // Slices a group's rows are cut into: about 128 rows each where the groups are even, four times as many where there
 // are several (one may hold much more than its share), and enough blocks to fill the GPU when there are few rows.
+// Up to eight slices are a cluster whose CTAs add their sums on chip, which saves the second kernel: the rule for up to
+// 1024 rows (512 x 1024: 6.1 us in two kernels; see slope_kernel).
 static uint32_t slope_slices(size_t M, size_t N, size_t G) {
+    if (M <= 1024) {
+        const uint32_t wanted = static_cast<uint32_t>((M + 63) / 64);
+        return wanted < 1 ? 1u : wanted > 8 ? 8u : wanted;
+    }
     const uint64_t spread = G < 4 ? G : 4;
     uint64_t slices = (M * spread + 128 * G - 1) / (128 * G);
     const uint64_t strips = ceil_div_u32(N, kSlopeColumns);
@@ -219,7 +262,18 @@ static size_t dz_bytes(size_t M, size_t N, const b200_linear_grads &g) {
 
 static size_t sums_bytes(size_t M, size_t N, size_t G, const b200_linear_grads &g) {
     const uint32_t slices = slope_slices(M, N, G);
-    return g.dbias && slices > 1 ? align256(static_cast<size_t>(slices) * G * N * sizeof(float)) : 0;
+    return g.dbias && slices > kSlopeCluster ? align256(static_cast<size_t>(slices) * G * N * sizeof(float)) : 0;
+}
+
+template <bool F32>
+static cudaError_t launch_slope_kernel(const cudaLaunchConfig_t *cfg, const SlopeParams &p, uint32_t act) {
+    switch (act) {
+        case kActRelu: return cudaLaunchKernelEx(cfg, slope_kernel<kActRelu, F32>, p);
+        case kActGelu: return cudaLaunchKernelEx(cfg, slope_kernel<kActGelu, F32>, p);
+        case kActGeluTanh: return cudaLaunchKernelEx(cfg, slope_kernel<kActGeluTanh, F32>, p);
+        case kActSilu: return cudaLaunchKernelEx(cfg, slope_kernel<kActSilu, F32>, p);
+        default: return cudaLaunchKernelEx(cfg, slope_kernel<kActNone, F32>, p);
+    }
 }
 
 static int launch_slope(const SlopeParams &p, uint32_t act, dim3 grid, cudaStream_t stream) {
@@ -231,14 +285,14 @@ static int launch_slope(const SlopeParams &p, uint32_t act, dim3 grid, cudaStrea
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = launch_attributes(attrs, 1);
-    cudaError_t e;
-    switch (act) {
-        case kActRelu: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActRelu>, p); break;
-        case kActGelu: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActGelu>, p); break;
-        case kActGeluTanh: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActGeluTanh>, p); break;
-        case kActSilu: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActSilu>, p); break;
-        default: e = cudaLaunchKernelEx(&cfg, slope_kernel<kActNone>, p); break;
+    if (p.clustered) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[cfg.numAttrs].val.clusterDim.x = 1;
+        attrs[cfg.numAttrs].val.clusterDim.y = p.slices;
+        attrs[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
     }
+    const cudaError_t e = p.c_type == B200_C_F32 ? launch_slope_kernel<true>(&cfg, p, act) : launch_slope_kernel<false>(&cfg, p, act);
     if (!cuda_ok(e, "cudaLaunchKernelEx")) return B200_HGEMM_ERR_CUDA;
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return B200_HGEMM_OK;
@@ -258,9 +312,10 @@ static int run_slope(const b200_linear_grads &g, void *dz, float *sums, const in
     p.slices = slope_slices(M, N, G);
     p.c_type = static_cast<uint32_t>(g.c_type);
     p.dz_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
-    const bool one = p.slices == 1;
+    const bool one = p.slices <= kSlopeCluster;  // one kernel does it all
     p.sums = g.dbias ? (one ? g.dbias : sums) : nullptr;
     p.accumulate = one && g.accumulate ? 1u : 0u;
+    p.clustered = g.dbias && one && p.slices > 1 ? 1u : 0u;
     const dim3 grid(ceil_div_u32(N, kSlopeColumns), p.slices, static_cast<unsigned>(G));
     int rc = launch_slope(p, static_cast<uint32_t>(g.act), grid, stream);
     if (rc != B200_HGEMM_OK || !g.dbias || one) return rc;

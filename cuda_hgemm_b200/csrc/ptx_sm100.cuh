@@ -57,6 +57,13 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
+// One float out of the shared memory of another CTA of the cluster.
+__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
 // Bulk copy from this CTA's shared memory into another CTA's of the cluster; the bytes are counted on a barrier
 // in the destination CTA. Both cluster addresses come from map_to_cta with the same rank; addresses and size
 // are multiples of 16 bytes. The source must stay allocated and unchanged until the destination's barrier has
@@ -457,6 +464,11 @@ __device__ __forceinline__ void tmem_ld_wait() {
 __device__ __forceinline__ uint32_t pack_half2_rn(uint32_t lo_f32_bits, uint32_t hi_f32_bits) {
     __half2 h = __floats2half2_rn(__uint_as_float(lo_f32_bits), __uint_as_float(hi_f32_bits));
     return *reinterpret_cast<uint32_t *>(&h);
+}
+
+// Asks for the line at `p` to be brought into L2; a hint, nothing is read.
+__device__ __forceinline__ void prefetch_l2(const void *p) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
 // L2-coherent (L1-bypassing) loads for data another CTA has just published.
