@@ -56,6 +56,7 @@ struct alignas(64) SkinnyParams {
     uint32_t n_pad;          // row pitch of the partial results, in floats
     uint32_t tma_store;      // 1: whole results leave through tm_c
     uint32_t prefetch_kb;    // k-blocks of B asked into L2 before waiting for the previous kernel
+    uint32_t after_all;      // host only: launch without overlap with the kernel before
     EpilogueArgs epi;        // kernels instantiated with EPI: alpha / beta / bias / c_in and the element type of C
 #ifdef B200_TIMELINE
     unsigned long long *timeline;  // profiling builds only: 32 words per CTA (see GemmParams::timeline)

@@ -230,13 +230,9 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
 // ---- the pass over dC -----------------------------------------------------------------------
 // Slices a group's rows are cut into: about 128 rows each where the groups are even, four times as many where there
 // are several (one may hold much more than its share), and enough blocks to fill the GPU when there are few rows.
-// Up to eight slices are a cluster whose CTAs add their sums on chip, which saves the second kernel: the rule for up to
-// 1024 rows (512 x 1024: 6.1 us in two kernels; see slope_kernel).
+// One slice, and no second kernel, for up to 64 rows: eight per warp.
 static uint32_t slope_slices(size_t M, size_t N, size_t G) {
-    if (M <= 1024) {
-        const uint32_t wanted = static_cast<uint32_t>((M + 63) / 64);
-        return wanted < 1 ? 1u : wanted > 8 ? 8u : wanted;
-    }
+    if (M <= 64) return 1u;
     const uint64_t spread = G < 4 ? G : 4;
     uint64_t slices = (M * spread + 128 * G - 1) / (128 * G);
     const uint64_t strips = ceil_div_u32(N, kSlopeColumns);
@@ -262,7 +258,7 @@ static size_t dz_bytes(size_t M, size_t N, const b200_linear_grads &g) {
 
 static size_t sums_bytes(size_t M, size_t N, size_t G, const b200_linear_grads &g) {
     const uint32_t slices = slope_slices(M, N, G);
-    return g.dbias && slices > kSlopeCluster ? align256(static_cast<size_t>(slices) * G * N * sizeof(float)) : 0;
+    return g.dbias && slices > 1 ? align256(static_cast<size_t>(slices) * G * N * sizeof(float)) : 0;
 }
 
 template <bool F32>
@@ -285,13 +281,6 @@ static int launch_slope(const SlopeParams &p, uint32_t act, dim3 grid, cudaStrea
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = launch_attributes(attrs, 1);
-    if (p.clustered) {
-        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attrs[cfg.numAttrs].val.clusterDim.x = 1;
-        attrs[cfg.numAttrs].val.clusterDim.y = p.slices;
-        attrs[cfg.numAttrs].val.clusterDim.z = 1;
-        ++cfg.numAttrs;
-    }
     const cudaError_t e = p.c_type == B200_C_F32 ? launch_slope_kernel<true>(&cfg, p, act) : launch_slope_kernel<false>(&cfg, p, act);
     if (!cuda_ok(e, "cudaLaunchKernelEx")) return B200_HGEMM_ERR_CUDA;
     g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -312,10 +301,9 @@ static int run_slope(const b200_linear_grads &g, void *dz, float *sums, const in
     p.slices = slope_slices(M, N, G);
     p.c_type = static_cast<uint32_t>(g.c_type);
     p.dz_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
-    const bool one = p.slices <= kSlopeCluster;  // one kernel does it all
+    const bool one = p.slices == 1;
     p.sums = g.dbias ? (one ? g.dbias : sums) : nullptr;
     p.accumulate = one && g.accumulate ? 1u : 0u;
-    p.clustered = g.dbias && one && p.slices > 1 ? 1u : 0u;
     const dim3 grid(ceil_div_u32(N, kSlopeColumns), p.slices, static_cast<unsigned>(G));
     int rc = launch_slope(p, static_cast<uint32_t>(g.act), grid, stream);
     if (rc != B200_HGEMM_OK || !g.dbias || one) return rc;

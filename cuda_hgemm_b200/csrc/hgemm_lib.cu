@@ -852,6 +852,7 @@ static int run_simt(const void *A, const void *B, void *C, size_t M, size_t N, s
 struct LibEpilogue : b200_hgemm_epilogue {
     uint32_t act = kActNone;
     uint32_t in_bf16 = 0;
+    bool linear = false;  // from b200_hgemm_linear
     void *pre = nullptr;
 };
 
@@ -1006,7 +1007,7 @@ static int launch_skinny_kernel(DeviceState &st, int attr_slot, const SkinnyPara
     cfg.stream = stream;
     cudaLaunchAttribute attrs[2];
     int n_attrs = 0;
-    if (pdl_enabled()) {
+    if (pdl_enabled() && !(CK && p.after_all)) {
         attrs[n_attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attrs[n_attrs].val.programmaticStreamSerializationAllowed = 1;
         ++n_attrs;
@@ -1061,6 +1062,10 @@ static int run_skinny(DeviceState &st, const void *A, const void *B, void *C, si
         const int erc = epilogue_args(*epi, &p.epi);
         if (erc != B200_HGEMM_OK) return erc;
     }
+    // Clusters of k-ranges in a linear layer start when the kernel before them has ended, not while it drains: they may
+    // follow the pair kernels of the gradients, and a kernel of small clusters launched programmatically behind one of
+    // those, another pair kernel behind it, has been seen never to end.
+    p.after_all = fused && epi->linear ? 1u : 0u;
     p.c = static_cast<__half *>(C);
     p.error_word = error_word;
     p.m = static_cast<uint32_t>(M);
@@ -1895,6 +1900,7 @@ int b200_hgemm_linear(const void *A, const void *B, void *C, size_t M, size_t N,
     epi.c_type = args->c_type;
     epi.act = static_cast<uint32_t>(args->act);
     epi.pre = args->pre;
+    epi.linear = true;
     epi.in_bf16 = args->in_type == B200_C_BF16 ? 1u : 0u;
     return run_plan(*st, A, B, C, M, N, K, pl, reinterpret_cast<cudaStream_t>(stream), need > 0 ? workspace : nullptr, workspace_bytes,
                     nullptr, &epi);

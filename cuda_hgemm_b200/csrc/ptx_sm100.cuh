@@ -57,13 +57,6 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
-// One float out of the shared memory of another CTA of the cluster.
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-    return v;
-}
-
 // Bulk copy from this CTA's shared memory into another CTA's of the cluster; the bytes are counted on a barrier
 // in the destination CTA. Both cluster addresses come from map_to_cta with the same rank; addresses and size
 // are multiples of 16 bytes. The source must stay allocated and unchanged until the destination's barrier has

@@ -8,8 +8,8 @@
 // warps take every eighth row, eight columns per lane, four rows in flight, which leaves registers for four blocks
 // on an SM. What is in flight is kept as it lies in memory: with the values already converted the same kernel
 // reached 2.3 TB/s. 8192 x 14336 in BF16: 142 us with gelu_tanh (705 MB, 4.9 TB/s), 167 us with gelu; eight rows
-// in flight 173 us, slices of 32 rows 173, of 512 rows 212. The slices' sums are added in order, by the first
-// CTA of a cluster that holds them or by bias_sum_kernel, so the result does not depend on timing.
+// in flight 173 us, slices of 32 rows 173, of 512 rows 212. The slices' sums are added in order by bias_sum_kernel,
+// so the result does not depend on timing.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -22,7 +22,6 @@ namespace b200 {
 
 constexpr int kSlopeThreads = 256;
 constexpr uint32_t kSlopeColumns = 256;
-constexpr uint32_t kSlopeCluster = 8;  // slices a cluster holds
 constexpr uint32_t kRowsInFlight = 4;  // 16-bit rows a warp has asked for before it uses the first (half as many of FP32)
 
 struct SlopeParams {
@@ -34,8 +33,7 @@ struct SlopeParams {
     uint32_t rows, n, groups, slices;
     uint32_t c_type;       // 0 FP16, 1 BF16, 2 FP32: type of dc and pre
     uint32_t dz_bf16;
-    uint32_t clustered;    // the slices of a strip are one cluster: its first CTA adds their sums and writes the gradient
-    uint32_t accumulate;   // slices == 1 or clustered: add to what `sums` holds
+    uint32_t accumulate;   // slices == 1: add to what `sums` holds
 };
 
 // Eight consecutive values of a row as they lie in memory (16 bytes, or 32 of FP32), and as FP32.
@@ -126,21 +124,10 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopePara
     for (int i = 0; i < 8; ++i) block_sums[warp][lane * 8 + i] = sum[i];
     __syncthreads();
     const uint32_t c = blockIdx.x * kSlopeColumns + threadIdx.x;
-    float total = 0.f;
+    if (c < p.n) {
+        float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSlopeThreads / 32; ++w) total += block_sums[w][threadIdx.x];
-    if (p.clustered) {
-        // every CTA leaves its sums in its own shared memory; the first reads them in order
-        block_sums[0][threadIdx.x] = total;  // (read by this thread alone so far)
-        cluster_sync_all();
-        if (slice == 0 && c < p.n) {
-            const uint32_t at = smem_u32(&block_sums[0][threadIdx.x]);
-            for (uint32_t s = 1; s < p.slices; ++s) total += ld_shared_cluster_f32(map_to_cta(at, s));
-            float *dst = p.sums + static_cast<size_t>(g) * p.n + c;
-            *dst = p.accumulate ? *dst + total : total;
-        }
-        cluster_sync_all();  // nobody's shared memory goes while it may be read
-    } else if (c < p.n) {
+        for (int w = 0; w < kSlopeThreads / 32; ++w) total += block_sums[w][threadIdx.x];
         float *dst = p.sums + (static_cast<size_t>(slice) * p.groups + g) * p.n + c;
         *dst = p.accumulate ? *dst + total : total;
     }
