@@ -57,6 +57,7 @@ constexpr uint32_t kGroupedMaxGroups = 1024;
 constexpr uint32_t kGroupedBand = 8;  // blocks of rows a band of tiles is high
 
 struct alignas(64) GroupedParams {
+    CUtensorMap tm_narrow[4];  // forward, kernels of 32 columns: as tm_p with boxes {64, 64}, {64, 80}, {64, 96}, {64, 112}
     CUtensorMap tm_p;     // forward {K, N, groups} box {64, 128}; input {K, N, groups} box {64, 64}; weight {N, T} box {64, 64} or
                           // {64, T, N / 64} box {64, 64, 2}
     CUtensorMap tm_q[8];  // forward {K, T}, input {N, T}: boxes {64, 16 (i + 1)}; weight: [0] = {K, T} as P
@@ -80,7 +81,6 @@ struct alignas(64) GroupedParams {
     uint32_t act;
     uint32_t accumulate;   // weight, FP32: add to the output
     uint32_t p_wide, q_wide;  // weight: the operand's map takes two boxes with one copy (load_columns)
-    FastDiv p_div;         // by p_blocks
 };
 
 template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG>
@@ -148,9 +148,9 @@ __device__ __forceinline__ void band_coord(uint32_t local, uint32_t nq, uint32_t
 
 // Forward and input form: tile id -> tile. off / cum: the table of offsets and of row blocks before each group.
 template <int CG>
-__device__ __forceinline__ void rows_tile(const GroupedParams &p, const uint32_t *off, const uint32_t *cum, uint32_t t,
-                                          GroupedTile &out) {
-    const uint32_t block = fast_div(t, p.p_div);
+__device__ __forceinline__ void rows_tile(const GroupedParams &p, const uint32_t *off, const uint32_t *cum, uint32_t p_blocks,
+                                          uint32_t width, uint32_t t, GroupedTile &out) {
+    const uint32_t block = t / p_blocks;
     uint32_t lo = 0, hi = p.groups;  // the largest g with cum[g] <= block; cum[groups] > block
     while (hi - lo > 1u) {
         const uint32_t mid = (lo + hi) >> 1;
@@ -159,10 +159,10 @@ __device__ __forceinline__ void rows_tile(const GroupedParams &p, const uint32_t
     const uint32_t first = cum[lo], nq = cum[lo + 1u] - first;
     const uint32_t start = off[lo], end = max(off[lo + 1u], start), r = end - start;
     uint32_t qb, pb;
-    band_coord(t - first * p.p_blocks, nq, p.p_blocks, &qb, &pb);
+    band_coord(t - first * p_blocks, nq, p_blocks, &qb, &pb);
     const uint32_t size = round_up_u32((r + nq - 1u) / nq, 16u * CG);  // even blocks
     out.group = lo;
-    out.p0 = pb * 128u * CG;
+    out.p0 = pb * width;
     out.q0 = start + qb * size;
     out.valid = min(size, r - qb * size);
     out.n_mma = round_up_u32(out.valid, 16u * CG);
@@ -239,7 +239,7 @@ __device__ __forceinline__ void store_transposed(void *out, uint32_t out_type, u
         float *dst = static_cast<float *>(out) + static_cast<size_t>(q0) * dim + col;
 #pragma unroll
         for (uint32_t j = 0; j < COUNT; ++j) {
-            if (j < valid && col < dim) dst[static_cast<size_t>(j) * dim] = __uint_as_float(r[j]);
+            if (j < valid) dst[static_cast<size_t>(j) * dim] = __uint_as_float(r[j]);
         }
         return;
     }
@@ -252,14 +252,14 @@ __device__ __forceinline__ void store_transposed(void *out, uint32_t out_type, u
             const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
             // even lane: row j of (this, next) column; odd lane: row j + 1 of (previous, this)
             const uint32_t word = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-            if (j + odd < valid && col < dim) dst[static_cast<size_t>(j) * (dim / 2u)] = word;
+            if (j + odd < valid) dst[static_cast<size_t>(j) * (dim / 2u)] = word;
         }
         return;
     }
     unsigned short *dst = static_cast<unsigned short *>(out) + static_cast<size_t>(q0) * dim + col;
 #pragma unroll
     for (uint32_t j = 0; j < COUNT; ++j) {
-        if (j < valid && col < dim) dst[static_cast<size_t>(j) * dim] = static_cast<unsigned short>(pack2_typed(r[j], r[j], out_type));
+        if (j < valid) dst[static_cast<size_t>(j) * dim] = static_cast<unsigned short>(pack2_typed(r[j], r[j], out_type));
     }
 }
 
@@ -273,12 +273,12 @@ __device__ __forceinline__ void add_residual(const void *residual, uint32_t type
     // would come back one at a time -- 28 us at 777 x 4099)
     if (type == 2u) {
 #pragma unroll
-        for (uint32_t j = 0; j < COUNT; ++j) v[j] = j < valid && col < dim ? static_cast<const float *>(residual)[at + static_cast<size_t>(j) * dim] : 0.f;
+        for (uint32_t j = 0; j < COUNT; ++j) v[j] = j < valid ? static_cast<const float *>(residual)[at + static_cast<size_t>(j) * dim] : 0.f;
     } else {
         unsigned short bits[COUNT];
 #pragma unroll
         for (uint32_t j = 0; j < COUNT; ++j) {
-            bits[j] = j < valid && col < dim ? static_cast<const unsigned short *>(residual)[at + static_cast<size_t>(j) * dim] : static_cast<unsigned short>(0);
+            bits[j] = j < valid ? static_cast<const unsigned short *>(residual)[at + static_cast<size_t>(j) * dim] : static_cast<unsigned short>(0);
         }
 #pragma unroll
         for (uint32_t j = 0; j < COUNT; ++j) v[j] = type == 1u ? __uint_as_float(static_cast<uint32_t>(bits[j]) << 16) : __half2float(__ushort_as_half(bits[j]));
@@ -290,7 +290,8 @@ __device__ __forceinline__ void add_residual(const void *residual, uint32_t type
 // What becomes of COUNT columns of an accumulator of the forward or input form.
 template <int FORM, int COUNT>
 __device__ __forceinline__ void finish_rows(const GroupedParams &p, uint32_t *r, float bias, uint32_t q0, uint32_t valid, uint32_t col,
-                                            uint32_t lane) {
+                                            uint32_t col_end, uint32_t lane) {
+    valid = col < col_end ? valid : 0u;  // (lanes without a column still take part in the exchanges)
     if (FORM == kFormForward) {
         if (p.bias) {
 #pragma unroll
@@ -372,7 +373,6 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
         tmem_alloc<CG>(smem_u32(const_cast<uint32_t *>(tmem_slot)), T::kTmemCols);
         tmem_relinquish<CG>();
     }
-    pdl_launch_dependents();
     pdl_wait_prior_grids();  // offsets and operands may have been written, and outputs read, by the previous kernel
 
     uint32_t tiles;
@@ -410,22 +410,48 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
     if (CG == 2) cluster_sync_all();  // the peer's copies and arrivals target this CTA's barriers
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
-    if (!WEIGHT) tiles = cum[p.groups] * p.p_blocks;
+    // Only now, with the kernel before this one complete: no more than two kernels of a chain are ever on the GPU.
+    pdl_launch_dependents();
+    // Columns of the result per tile. Where a tile takes few rows its time is that of reading its weights, and the
+    // kernel's that of the SM with the most of them: 26 groups of 1024 columns are 208 tiles of 128, two for an SM, or 286 of
+    // 96, two for an SM as well. The width with the least waves x (width + the rows' share of a stage and a tile's fixed
+    // cost, about 40 columns' worth) is taken; the MMA's other rows multiply what lies in the slab and are not stored.
+    uint32_t width = 128u * CG, p_blocks = p.p_blocks;
+    if (!WEIGHT) {
+        const uint32_t row_blocks = cum[p.groups];
+        if (QT == 32) {
+            uint32_t least = 0xffffffffu;
+            for (uint32_t w = 128u; w >= 64u; w -= FORM == kFormForward ? 16u : 64u) {
+                const uint32_t n = (p.p_dim + w - 1u) / w;
+                const uint32_t cost = (row_blocks * n + workers - 1u) / workers * (w + 40u);
+                if (cost < least) {
+                    least = cost;
+                    width = w;
+                    p_blocks = n;
+                }
+            }
+        }
+        tiles = row_blocks * p_blocks;
+    }
+    const CUtensorMap *p_map = QT == 32 && FORM == kFormForward && width < 128u ? &p.tm_narrow[width / 16u - 4u] : &p.tm_p;
+    const uint32_t p_bytes = QT == 32 ? width * 128u : T::kPBytes;  // of a slab of P, as staged
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
-        if (lane == 0) {
+        bool chosen;
+        elect_lane(&chosen);
+        if (chosen) {
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (uint32_t t = worker; ok && t < tiles; t += workers) {
                 GroupedTile tile;
-                if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
+                if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, p_blocks, width, t, tile);
                 const uint32_t blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks;
                 const uint32_t q_rows = tile.n_mma / CG;  // forward, input: rows this CTA stages
                 const int32_t p_at = static_cast<int32_t>(tile.p0 + cta_rank * 128u);
                 const int32_t q_at = static_cast<int32_t>(tile.q0 + cta_rank * q_rows);
                 const CUtensorMap *q_map = &p.tm_q[WEIGHT ? 0u : q_rows / 16u - 1u];
-                const uint32_t bytes = KPS * (T::kPBytes + (WEIGHT ? T::kQBytes : q_rows * 128u));
+                const uint32_t bytes = KPS * (p_bytes + (WEIGHT ? T::kQBytes : q_rows * 128u));
                 const uint32_t rest = WEIGHT ? (tile.valid & (kStepK - 1u)) : 0u;  // rows of a tail, 0: whole blocks
                 const uint32_t whole = blocks - (rest != 0 ? 1u : 0u);
                 for (uint32_t kb = 0; kb < whole; ++kb) {
@@ -454,10 +480,11 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                         } else {
                             const int32_t g = static_cast<int32_t>(tile.group);
                             if (FORM == kFormForward) {
-                                if (CG == 2) tma_load_3d_pair(sp, &p.tm_p, kx, p_at, g, bar); else tma_load_3d(sp, &p.tm_p, kx, p_at, g, bar);
+                                if (CG == 2) tma_load_3d_pair(sp, p_map, kx, p_at, g, bar); else tma_load_3d(sp, p_map, kx, p_at, g, bar);
                             } else {
 #pragma unroll
                                 for (int32_t h = 0; h < 2; ++h) {
+                                    if (QT == 32 && h == 1 && width < 128u) break;
                                     if (CG == 2) tma_load_3d_pair(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
                                     else tma_load_3d(sp + h * 8192u, &p.tm_p, p_at + h * 64, kx, g, bar);
                                 }
@@ -499,6 +526,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
         // ------------------------------------------------------------------ MMA issuer
         // The whole warp walks the tiles; one lane of the leader issues. In the weight form all lanes clear the lines
         // of a tail (in both CTAs of a pair).
+        bool chosen;
+        const uint32_t issuer = elect_lane(&chosen);
         if (cta_rank == 0 || WEIGHT) {
             const uint32_t idesc_base = umma_idesc_f16_f32(128 * CG, 0) | (P_MN ? kUmmaIdescAMn : 0u) | (WEIGHT ? (1u << 16) : 0u) |
                                         (p.in_bf16 ? kUmmaIdescBf16 : 0u);
@@ -507,14 +536,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
             bool ok = true;
             for (uint32_t t = worker; ok && t < tiles; t += workers) {
                 GroupedTile tile;
-                if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
+                if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, p_blocks, width, t, tile);
                 const uint32_t blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks;
                 if (blocks == 0) continue;
                 const uint32_t rest = WEIGHT ? (tile.valid & (kStepK - 1u)) : 0u;  // rows of a tail, 0: whole blocks
                 const uint32_t idesc = idesc_base | ((tile.n_mma >> 3) << 17);
                 const uint32_t whole = blocks - (rest != 0 ? 1u : 0u);
                 uint32_t d_tmem = tmem_base + (it & 1u) * QT;
-                if (cta_rank == 0 && lane == 0) {
+                if (cta_rank == 0 && chosen) {
                     if (!mbar_wait(tempty_bar + 8u * (it & 1u), ((it >> 1) & 1u) ^ 1u, abort_flag)) ok = false;
                     tcgen05_fence_after_sync();
                     uint32_t begun = 0;  // 1: the accumulator holds a part of this piece
@@ -558,23 +587,23 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 }
                 if constexpr (WEIGHT) {
                     // every lane follows: where the ring stands, and whether to go on
-                    ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
-                    it = __shfl_sync(0xffffffffu, it, 0);
+                    ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, issuer) != 0;
+                    it = __shfl_sync(0xffffffffu, it, issuer);
                     if (CG == 2 && cta_rank != 0) {
                         const uint32_t at = stage + blocks - (rest != 0 ? 1u : 0u);
                         stage = at % STAGES;
                         phase ^= (at / STAGES) & 1u;
                     } else {
-                        stage = __shfl_sync(0xffffffffu, stage, 0);
-                        phase = __shfl_sync(0xffffffffu, phase, 0);
+                        stage = __shfl_sync(0xffffffffu, stage, issuer);
+                        phase = __shfl_sync(0xffffffffu, phase, issuer);
                     }
                     if (ok && rest != 0) {
                         const uint32_t slot = base + stage * T::kStageBytes;
                         const uint32_t landed_bar = (CG == 2 ? tail_bar : full_bar) + 8u * stage;
                         const uint32_t parity = CG == 2 ? (tail_phase >> stage) & 1u : phase;
                         uint32_t landed = 1;
-                        if (lane == 0) landed = mbar_wait(landed_bar, parity, abort_flag) ? 1u : 0u;
-                        landed = __shfl_sync(0xffffffffu, landed, 0);
+                        if (chosen) landed = mbar_wait(landed_bar, parity, abort_flag) ? 1u : 0u;
+                        landed = __shfl_sync(0xffffffffu, landed, issuer);
                         if (landed) {
                             // each lane passes the completed barrier itself: the copies' bytes are then ordered before its stores
                             mbar_try_wait(landed_bar, parity);
@@ -588,7 +617,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                             }
                             fence_proxy_async_smem();
                             __syncwarp();
-                            if (lane == 0) {
+                            if (chosen) {
                                 if (CG == 2) mbar_arrive_cluster(map_to_cta(ready_bar + 8u * stage, 0));
                                 if (cta_rank == 0) {
                                     if (CG == 2) {
@@ -614,7 +643,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                         } else {
                             ok = false;
                         }
-                        ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+                        ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, issuer) != 0;
                         tail_phase ^= 1u << stage;
                         if (++stage == STAGES) {
                             stage = 0;
@@ -622,12 +651,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                         }
                     }
                 }
-                if (cta_rank == 0 && lane == 0 && ok) {
+                if (cta_rank == 0 && chosen && ok) {
                     if (CG == 1) umma_commit(tfull_bar + 8u * (it & 1u)); else umma_commit_pair(tfull_bar + 8u * (it & 1u), 0x3);
                 }
                 if (!WEIGHT) {
-                    ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
-                    it = __shfl_sync(0xffffffffu, it, 0);
+                    ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, issuer) != 0;
+                    it = __shfl_sync(0xffffffffu, it, issuer);
                 }
                 ++it;
             }
@@ -662,15 +691,16 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
         };
         for (uint32_t t = worker; alive && t < tiles; t += workers) {
             GroupedTile tile;
-            if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, t, tile);
+            if (WEIGHT) weight_tile<CG, QT>(p, t, tile); else rows_tile<CG>(p, off, cum, p_blocks, width, t, tile);
             const bool summed = !WEIGHT || tile.valid != 0;  // a group without rows: a gradient of zeros, no accumulator
             const uint32_t p_warp = tile.p0 + cta_rank * 128u + q * 32u;  // first index on P of this warp's lanes
             const uint32_t lanes = tmem_base + ((q * 32u) << 16);
             const uint32_t cols = WEIGHT ? min(static_cast<uint32_t>(QT), p.q_dim - tile.q0) : tile.valid;  // columns stored
-            const bool live = p_warp < p.p_dim && (summed || !p.accumulate);
-            const uint32_t col = p_warp + lane;  // forward, input: this lane's output column
+            // forward, input: this lane's output column, and where the columns of this tile end
+            const uint32_t col = p_warp + lane, col_end = QT == 32 ? min(p.p_dim, tile.p0 + width) : p.p_dim;
+            const bool live = p_warp < col_end && (summed || !p.accumulate);
             float bias = 0.f;
-            if (FORM == kFormForward && p.bias && col < p.p_dim) {
+            if (FORM == kFormForward && p.bias && col < col_end) {
                 const size_t at = static_cast<size_t>(tile.group) * p.p_dim + col;
                 bias = p.in_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[at])
                                  : __half2float(static_cast<const __half *>(p.bias)[at]);
@@ -719,9 +749,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 if (live) {
                     if constexpr (LONG) {
 #pragma unroll
-                        for (uint32_t i = 0; i < kChunks; ++i) {
-                            const uint32_t at = (2u * i + half) * W;
-                            if (at < cols) finish_rows<FORM, W>(p, run + i * W, bias, tile.q0 + at, cols - at, col, lane);
+                        for (uint32_t i = 0; i < kChunks * W / 16u; ++i) {  // (16 at a time: the running sums leave few registers)
+                            const uint32_t at = (2u * (i * 16u / W) + half) * W + i * 16u % W;
+                            if (at < cols) finish_rows<FORM, 16>(p, run + i * 16u, bias, tile.q0 + at, cols - at, col, col_end, lane);
                         }
                     } else {
 #pragma unroll 1
@@ -729,7 +759,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                             uint32_t r[W];
                             tmem_ld_columns<W>(taddr + at, r);
                             tmem_ld_wait();
-                            finish_rows<FORM, W>(p, r, bias, tile.q0 + at, cols - at, col, lane);
+                            finish_rows<FORM, W>(p, r, bias, tile.q0 + at, cols - at, col, col_end, lane);
                         }
                     }
                 }

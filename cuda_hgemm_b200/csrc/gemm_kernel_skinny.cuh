@@ -10,7 +10,8 @@
 // column operand (UMMA 128 x MT x 16), and the accumulator holds C transposed: tensor-memory lane = column
 // of C, tensor-memory column = row of C. A stage is two k-blocks (32 KB of B and 2 x MT x 128 B of A)
 // under one barrier round trip, six stages deep for MT = 16: twice the bytes of B in flight per SM and
-// 0.20 us of issue time per k-block. One CTA computes one (column tile, k-range) pair; when the tiles
+// little more than 0.10 us of issue time per k-block (0.20 us before the issuing lanes were elected, see elect_lane:
+// M = 16 at N = 14336 from 21.1 to 20.4 us inside a graph, M = 16 at N = 4096, K = 14336 from 21.9 to 20.9). One CTA computes one (column tile, k-range) pair; when the tiles
 // are too few to fill the GPU (N = 4096: 32) the k-range is cut into equal slices. Their FP32 partial
 // results are summed either inside a thread-block cluster that holds the k-ranges of one tile (template
 // parameter CK below: no workspace, no second kernel) or, for more k-ranges than a cluster takes, through a
@@ -209,7 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
-        if (lane == 0) {
+        bool chosen;
+        elect_lane(&chosen);
+        if (chosen) {
             uint32_t stage = 0, phase = 0;
             const uint32_t block_tx = p.tile_w * kBK * 2u + T::kXBytes;  // bytes one CTA stages per k-block
             const int32_t row_x = static_cast<int32_t>(cta_rank * T::kXRows);
@@ -255,7 +258,9 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
-        if (lane == 0 && cta_rank == 0) {
+        bool chosen;
+        elect_lane(&chosen);
+        if (chosen && cta_rank == 0) {
             const uint32_t idesc = umma_idesc_f16_f32(128 * CG, MT) | (EPI && p.epi.in_bf16 ? kUmmaIdescBf16 : 0u);
             uint32_t stage = 0, phase = 0;
             bool ok = true;

@@ -27,10 +27,13 @@ static bool misaligned(std::initializer_list<const void *> ptrs) {
     return (bits & 15u) != 0;
 }
 
-// Kernel attributes of one launch: programmatic dependent launch, and the pair where there is one.
-static int launch_attributes(cudaLaunchAttribute *attrs, int cg) {
+// Kernel attributes of one launch: programmatic dependent launch where `overlap` allows it, and the pair where there is
+// one. The pass over dC starts behind the kernel before it, and a product behind that pass, without overlap: the
+// small CTAs of the one and the whole-SM pairs of the other, started early and waiting beside each other, have
+// been seen to stand still for good. Between two products the overlap stays.
+static int launch_attributes(cudaLaunchAttribute *attrs, int cg, bool overlap) {
     int n = 0;
-    if (pdl_enabled()) {
+    if (overlap && pdl_enabled()) {
         attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attrs[n].val.programmaticStreamSerializationAllowed = 1;
         ++n;
@@ -48,7 +51,7 @@ static int launch_attributes(cudaLaunchAttribute *attrs, int cg) {
 // `most_tiles`: an upper bound of the tiles there can be; the grid is persistent and never larger than what
 // is resident at once.
 template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG = false>
-static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uint64_t most_tiles, cudaStream_t stream) {
+static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uint64_t most_tiles, bool overlap, cudaStream_t stream) {
     using T = GroupedTraits<FORM, CG, QT, STAGES, KPS, LONG>;
     auto kern = hgemm_grouped_kernel<FORM, CG, QT, STAGES, KPS, LONG>;
     cudaLaunchConfig_t cfg;
@@ -58,7 +61,7 @@ static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uin
     cfg.dynamicSmemBytes = T::kSmemBytes;
     cfg.stream = stream;
     cfg.attrs = attrs;
-    cfg.numAttrs = launch_attributes(attrs, CG);
+    cfg.numAttrs = launch_attributes(attrs, CG, overlap);
     uint32_t resident = static_cast<uint32_t>(st.sm_count);
     {
         std::lock_guard<std::mutex> lock(st.mu);
@@ -102,20 +105,19 @@ struct RowsPlan {
 };
 
 // The kernel and the most rows per block that should take the least time: waves of tiles times the time of one.
-// A k-block of a tile takes the longest of what the issuing thread needs (0.28 us with one k-block to a stage, 0.20
-// with two), the MMAs (0.27 us for 128 x 256 outputs per CTA) and the operands' way from L2 (11.5 TB/s for all
-// SMs together: what tiles of few rows run into); the start costs about 3 us, 1.2 more where two CTAs have to meet, and
-// the last epilogue 12 ns a row. Group sizes are not known here: the estimate spreads the rows evenly over the groups. Measured
-// over 25 shapes with every kernel and height forced, the choice was the fastest or within 5 percent of it in all but
-// three (10 percent); e.g. 777 x 4099 x 2056: pairs with blocks of 224 rows 24.6 us, single CTAs 33.5; 512 x 4096 x
-// 14336: pairs with 128 rows 58.8, with 256 rows 75.7; 200 x 1024 x 1024: single CTAs 8.1, pairs 9.8.
+// Measured with one to 144 CTAs at work (K = 2048 against 8192), a k-block of a tile takes the longest of
+//   * what the issuing threads need: 0.14 us for single CTAs, 0.10 for pairs and for blocks of 32 rows,
+//   * its MMAs: 1.1 ns per row of the block (1.3 with the whole GPU at work), 128 columns of the result per CTA,
+//   * its operands' way out of L2: 20.5 TB/s for all SMs together;
+// a kernel costs 4 us besides (5.5 where two CTAs have to meet), and 10 ns per row of a block for the last
+// epilogue. Group sizes are not known here: the estimate spreads the rows evenly over the groups.
 static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_dim, size_t k_dim, size_t groups) {
     const uint64_t live = groups < rows ? groups : rows;  // groups that can hold any rows
     const uint64_t average = (rows + live - 1) / live;
     RowsPlan best{kRowsSingle32, 32};
     if (average <= 32) return best;
     double best_us = 1e30;
-    for (uint32_t kernel = kRowsPair256; kernel <= kRowsSingle128; ++kernel) {
+    for (uint32_t kernel = kRowsPair256; kernel <= kRowsSingle32; ++kernel) {
         const RowsKernelShape &shape = rows_kernels[kernel];
         const double slots = st.sm_count / shape.cg;
         for (uint32_t q_max = shape.q_cap; q_max >= 32u; q_max -= 32u) {
@@ -124,13 +126,12 @@ static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_di
             const double q = static_cast<double>((average + blocks - 1) / blocks);
             const double tiles = static_cast<double>(blocks * live) * ceil_div_u32(p_dim, 128u * shape.cg);
             const double active = tiles < slots ? tiles : slots;
-            const double operands = active * shape.cg * (16384.0 + q / shape.cg * 128.0);
-            double per_block = operands / 11.5e6;
-            const double mma = 0.27 * q / 256.0, issue = shape.kps == 2 ? 0.20 : 0.28;
+            double per_block = active * shape.cg * (16384.0 + q / shape.cg * 128.0) / 20.5e6;
+            const double mma = (active * shape.cg > 100.0 ? 0.0013 : 0.0011) * q;
+            const double issue = kernel == kRowsSingle128 ? 0.14 : 0.10;
             if (per_block < mma) per_block = mma;
             if (per_block < issue) per_block = issue;
-            const double waves = ceil(tiles / slots);
-            const double us = waves * per_block * ceil_div_u32(k_dim, 64) + (shape.cg == 2 ? 4.2 : 3.0) + 0.012 * q;
+            const double us = ceil(tiles / slots) * per_block * ceil_div_u32(k_dim, 64) + (shape.cg == 2 ? 5.5 : 4.0) + 0.010 * q;
             if (us < best_us * 0.999) {
                 best_us = us;
                 best = RowsPlan{kernel, q_max};
@@ -143,7 +144,7 @@ static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_di
 // Forward and input form. X: the rows' operand [rows x k_dim]; W: groups matrices [w_rows x w_cols], stride_w apart.
 template <int FORM>
 static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, size_t p_dim, size_t k_dim, size_t w_rows,
-                    size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, cudaStream_t stream) {
+                    size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, bool overlap, cudaStream_t stream) {
     constexpr int kSlots = FORM == kFormForward ? 96 : 104;
     p.error_word = st.error_word;
     p.rows = static_cast<uint32_t>(rows);
@@ -153,14 +154,19 @@ static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, 
     const int cg = rows_kernels[plan.kernel].cg, kps = rows_kernels[plan.kernel].kps;
     p.q_max = plan.q_max;
     p.p_blocks = ceil_div_u32(p_dim, 128u * cg);
-    p.p_div = make_fast_div(p.p_blocks);
     p.k_blocks = ceil_div_u32(k_dim, 64u * kps);
-    // an upper bound: every group may end in a block that is not full
-    const uint64_t tiles = (rows / p.q_max + (groups < rows ? groups : rows)) * p.p_blocks;
+    // an upper bound: every group may end in a block that is not full, and tiles may be as narrow as 64
+    const uint64_t tiles = (rows / p.q_max + (groups < rows ? groups : rows)) *
+                           (plan.kernel == kRowsSingle32 ? ceil_div_u32(p_dim, 64) : p.p_blocks);
     if (tiles > 0x7fffffffull) return B200_HGEMM_ERR_TOO_LARGE;
     int rc;
     const uint32_t box_rows = FORM == kFormForward ? 128u : 64u;
     if ((rc = get_tensor_map(st, W, w_rows, w_cols, box_rows, 64, &p.tm_p, true, groups, stride_w)) != B200_HGEMM_OK) return rc;
+    if (FORM == kFormForward && plan.kernel == kRowsSingle32) {
+        for (uint32_t i = 0; i < 4; ++i) {
+            if ((rc = get_tensor_map(st, W, w_rows, w_cols, 64u + 16u * i, 64, &p.tm_narrow[i], true, groups, stride_w)) != B200_HGEMM_OK) return rc;
+        }
+    }
     for (uint32_t i = 0; i < p.q_max / (16u * cg); ++i) {
         if ((rc = get_tensor_map(st, X, rows, k_dim, 16u * (i + 1u), 64, &p.tm_q[i])) != B200_HGEMM_OK) return rc;
     }
@@ -168,18 +174,18 @@ static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, 
     if constexpr (FORM == kFormForward) {
         if (p.out_type == B200_C_F32 && k_dim > kLongSum) {
             switch (plan.kernel) {
-                case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, stream);
-                case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, stream);
-                case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, stream);
-                default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, stream);
+                case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, overlap, stream);
+                case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, overlap, stream);
+                case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, overlap, stream);
+                default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, overlap, stream);
             }
         }
     }
     switch (plan.kernel) {
-        case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1>(st, slot, p, tiles, stream);
-        case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2>(st, slot, p, tiles, stream);
-        case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2>(st, slot, p, tiles, stream);
-        default: return launch_grouped<FORM, 1, 32, 5, 2>(st, slot, p, tiles, stream);
+        case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1>(st, slot, p, tiles, overlap, stream);
+        case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2>(st, slot, p, tiles, overlap, stream);
+        case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2>(st, slot, p, tiles, overlap, stream);
+        default: return launch_grouped<FORM, 1, 32, 5, 2>(st, slot, p, tiles, overlap, stream);
     }
 }
 
@@ -192,9 +198,26 @@ static int columns_map(DeviceState &st, const void *ptr, size_t rows, size_t wid
     return get_tensor_map(st, ptr, rows, width, 64, 64, map);
 }
 
+// Weight form: pairs on 256 x 256 or single CTAs on 128 x 128, by the estimate of choose_rows_plan (single CTAs need 0.16 us
+// per block of 64 rows, pairs 0.28).
+static int weight_cg(const DeviceState &st, size_t M, size_t N, size_t K, size_t G) {
+    const double blocks = ceil_div_u32((M + G - 1) / G, 64);
+    double us[2];
+    for (int cg = 1; cg <= 2; ++cg) {
+        const double slots = st.sm_count / cg;
+        const double tiles = static_cast<double>(G) * ceil_div_u32(N, 128u * cg) * ceil_div_u32(K, 128u * cg);
+        const double active = tiles < slots ? tiles : slots;
+        double per_block = active * cg * 32768.0 / 20.5e6;
+        const double least = cg == 1 ? 0.16 : active > 50.0 ? 0.33 : 0.28;
+        if (per_block < least) per_block = least;
+        us[cg - 1] = ceil(tiles / slots) * (per_block * blocks + (cg == 1 ? 1.0 : 2.0)) + (cg == 1 ? 4.0 : 5.5);
+    }
+    return us[1] < us[0] ? 2 : 1;
+}
+
 // Weight form: dB_g = dZ_g^T A_g.
 static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, const int32_t *offsets, size_t M, size_t N, size_t K,
-                      size_t G, const b200_linear_grads &g, cudaStream_t stream) {
+                      size_t G, const b200_linear_grads &g, bool overlap, cudaStream_t stream) {
     GroupedParams p;
     memset(&p, 0, sizeof(p));
     p.out = dB;
@@ -207,11 +230,9 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
     p.in_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
     p.out_type = static_cast<uint32_t>(g.db_type);
     p.accumulate = g.accumulate ? 1u : 0u;
-    const uint64_t pair_tiles = static_cast<uint64_t>(G) * ceil_div_u32(N, 256) * ceil_div_u32(K, 256);
-    const int cg = pair_tiles >= static_cast<uint64_t>(st.sm_count) / 2 ? 2 : 1;
+    const int cg = weight_cg(st, M, N, K, G);
     p.p_blocks = ceil_div_u32(N, 128u * cg);
     p.q_blocks = ceil_div_u32(K, 128u * cg);
-    p.p_div = make_fast_div(p.p_blocks);
     const uint64_t tiles = static_cast<uint64_t>(G) * p.p_blocks * p.q_blocks;
     if (tiles > 0x7fffffffull) return B200_HGEMM_ERR_TOO_LARGE;
     int rc;
@@ -220,11 +241,11 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
     const bool f32 = g.db_type == B200_C_F32;
     if ((rc = get_tensor_map(st, dB, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
     if (f32 && M > kLongSum) {
-        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, stream);
-        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, stream);
+        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, overlap, stream);
+        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, overlap, stream);
     }
-    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 110, p, tiles, stream);
-    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, stream);
+    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 110, p, tiles, overlap, stream);
+    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, overlap, stream);
 }
 
 // ---- the pass over dC -----------------------------------------------------------------------
@@ -280,7 +301,7 @@ static int launch_slope(const SlopeParams &p, uint32_t act, dim3 grid, cudaStrea
     cfg.blockDim = dim3(kSlopeThreads, 1, 1);
     cfg.stream = stream;
     cfg.attrs = attrs;
-    cfg.numAttrs = launch_attributes(attrs, 1);
+    cfg.numAttrs = launch_attributes(attrs, 1, false);
     const cudaError_t e = p.c_type == B200_C_F32 ? launch_slope_kernel<true>(&cfg, p, act) : launch_slope_kernel<false>(&cfg, p, act);
     if (!cuda_ok(e, "cudaLaunchKernelEx")) return B200_HGEMM_ERR_CUDA;
     g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -315,7 +336,7 @@ static int run_slope(const b200_linear_grads &g, void *dz, float *sums, const in
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
     cfg.attrs = attrs;
-    cfg.numAttrs = launch_attributes(attrs, 1);
+    cfg.numAttrs = launch_attributes(attrs, 1, true);
     if (!cuda_ok(cudaLaunchKernelEx(&cfg, bias_sum_kernel, static_cast<const float *>(sums), g.dbias, count, p.slices,
                                     g.accumulate ? 1u : 0u),
                  "cudaLaunchKernelEx")) {
@@ -356,7 +377,7 @@ static GroupedParams forward_params(void *C, const int32_t *offsets, const b200_
 int run_linear_rows(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args &args,
                     cudaStream_t stream) {
     GroupedParams p = forward_params(C, nullptr, args);
-    return run_rows<kFormForward>(st, A, B, M, N, K, N, K, 1, N * K, p, stream);
+    return run_rows<kFormForward>(st, A, B, M, N, K, N, K, 1, N * K, p, true, stream);
 }
 
 static int grouped_forward(const void *A, const void *B, void *C, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
@@ -373,7 +394,7 @@ static int grouped_forward(const void *A, const void *B, void *C, const int32_t 
     if ((rc = current_state(&st)) != B200_HGEMM_OK) return rc;
     if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
     GroupedParams p = forward_params(C, offsets, *args);
-    return run_rows<kFormForward>(*st, A, B, M, N, K, N, K, G, G > 1 ? stride_b : N * K, p, stream);
+    return run_rows<kFormForward>(*st, A, B, M, N, K, N, K, G, G > 1 ? stride_b : N * K, p, true, stream);
 }
 
 // Both backward entry points; `offsets` is null for the dense one.
@@ -410,7 +431,8 @@ static int backward(const void *A, const void *B, const int32_t *offsets, size_t
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     void *dz = g.dZ ? g.dZ : (need_dz ? ws : nullptr);
     float *sums = reinterpret_cast<float *>(ws + need_dz);
-    if (dz || g.dbias) {
+    bool passed = dz || g.dbias;  // the next product follows the pass over dC
+    if (passed) {
         if ((rc = run_slope(g, dz, sums, offsets, M, N, G, stream)) != B200_HGEMM_OK) return rc;
     }
     const void *dz_read = needs_dz(g) ? dz : g.dC;
@@ -421,10 +443,11 @@ static int backward(const void *A, const void *B, const int32_t *offsets, size_t
         p.offsets = offsets;
         p.in_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
         p.out_type = static_cast<uint32_t>(g.in_type);
-        rc = run_rows<kFormInput>(*st, dz_read, B, M, K, N, N, K, G, G > 1 ? stride_b : N * K, p, stream);
+        rc = run_rows<kFormInput>(*st, dz_read, B, M, K, N, N, K, G, G > 1 ? stride_b : N * K, p, !passed, stream);
+        passed = false;
         if (rc != B200_HGEMM_OK) return rc;
     }
-    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, stream);
+    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, !passed, stream);
     return B200_HGEMM_OK;
 }
 

@@ -61,8 +61,8 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopePara
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t col = blockIdx.x * kSlopeColumns + lane * 8u;
     const uint32_t slice = blockIdx.y, g = blockIdx.z;
-    pdl_launch_dependents();
     pdl_wait_prior_grids();
+    pdl_launch_dependents();
     uint32_t start = 0, end = p.rows;
     if (p.offsets) {
         const int32_t a = __ldg(p.offsets + g), b = __ldg(p.offsets + g + 1);
@@ -135,7 +135,6 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopePara
 
 // dbias[i] = sum of the slices' sums, in order (added to what is there with `accumulate`).
 __global__ void __launch_bounds__(256) bias_sum_kernel(const float *sums, float *dbias, size_t count, uint32_t slices, uint32_t accumulate) {
-    pdl_launch_dependents();
     pdl_wait_prior_grids();
     const size_t i = static_cast<size_t>(blockIdx.x) * 256u + threadIdx.x;
     if (i >= count) return;

@@ -137,7 +137,7 @@ def check_backward(dC, A, B, act, pre, dZ, dA, dB, dbias, what, dB_was=None, dbi
 # ------------------------------------------------------------------------------------------------ linear, forward
 LINEAR_SHAPES = [
     (1, 8, 8), (1, 64, 72), (3, 1, 16), (16, 1024, 512), (17, 33, 40), (64, 4099, 136), (16, 4096, 4096), (100, 512, 4096),
-    (128, 4096, 1024), (129, 257, 64), (300, 700, 200), (777, 1000, 520), (1024, 2048, 256),
+    (128, 4096, 1024), (128, 4096, 8192), (40, 1024, 4096), (129, 257, 64), (300, 700, 200), (777, 1000, 520), (1024, 2048, 256),
 ]
 
 
