@@ -80,6 +80,7 @@ struct alignas(64) GroupedParams {
     uint32_t out_type;     // 0 FP16, 1 BF16, 2 FP32
     uint32_t act;
     uint32_t accumulate;   // weight, FP32: add to the output
+    uint32_t slice_rows;   // weight, dense: "group" g is rows [g, g + 1) * slice_rows of one long sum (0: groups as `offsets` says)
     uint32_t p_wide, q_wide;  // weight: the operand's map takes two boxes with one copy (load_columns)
 };
 
@@ -180,6 +181,9 @@ __device__ __forceinline__ void weight_tile(const GroupedParams &p, uint32_t t, 
     if (p.offsets) {
         start = held_offset(__ldg(p.offsets + g), p.rows);
         end = max(held_offset(__ldg(p.offsets + g + 1), p.rows), start);
+    } else if (p.slice_rows) {
+        start = g * p.slice_rows;  // (every slice holds rows: start < rows)
+        end = min(start + p.slice_rows, p.rows);
     }
     out.group = g;
     out.p0 = pb * 128u * CG;

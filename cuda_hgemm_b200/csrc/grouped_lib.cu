@@ -199,7 +199,8 @@ static int columns_map(DeviceState &st, const void *ptr, size_t rows, size_t wid
 }
 
 // Weight form: pairs on 256 x 256 or single CTAs on 128 x 128, by the estimate of choose_rows_plan (single CTAs need 0.16 us
-// per block of 64 rows, pairs 0.28).
+// per block of 64 rows, pairs 0.28; a tile costs 1.0 and 2.8 us besides, which decides for groups of few rows: 32 groups
+// of 128 rows, 1024 x 2048 in FP16, 38 us on single CTAs and 48 on pairs).
 static int weight_cg(const DeviceState &st, size_t M, size_t N, size_t K, size_t G) {
     const double blocks = ceil_div_u32((M + G - 1) / G, 64);
     double us[2];
@@ -210,27 +211,57 @@ static int weight_cg(const DeviceState &st, size_t M, size_t N, size_t K, size_t
         double per_block = active * cg * 32768.0 / 20.5e6;
         const double least = cg == 1 ? 0.16 : active > 50.0 ? 0.33 : 0.28;
         if (per_block < least) per_block = least;
-        us[cg - 1] = ceil(tiles / slots) * (per_block * blocks + (cg == 1 ? 1.0 : 2.0)) + (cg == 1 ? 4.0 : 5.5);
+        us[cg - 1] = ceil(tiles / slots) * (per_block * blocks + (cg == 1 ? 1.0 : 2.8)) + (cg == 1 ? 4.0 : 5.5);
     }
     return us[1] < us[0] ? 2 : 1;
 }
 
+// Slices a dense layer's long sum over the rows is cut into where its gradient has too few tiles for the GPU: as many as
+// give every SM a tile, of at least 512 rows each. They lie in FP32 in the workspace (20 MB at most) and slice_sum_kernel
+// adds them in order. 8192 rows of 256 x 256: 31 us in one piece, 10 in sixteen.
+static uint32_t weight_slices(size_t M, size_t N, size_t K, size_t G, bool ragged) {
+    constexpr uint64_t kSms = 148;  // (of a B200; the workspace size must not depend on the current device)
+    if (ragged || G != 1 || M < 1024) return 1;
+    const uint64_t tiles = static_cast<uint64_t>(ceil_div_u32(N, 128)) * ceil_div_u32(K, 128);
+    const uint64_t slices = kSms / tiles < M / 512 ? kSms / tiles : M / 512;
+    return slices < 2 ? 1u : static_cast<uint32_t>(slices);
+}
+
+static size_t align256(size_t v) {
+    return (v + 255) / 256 * 256;
+}
+
+static size_t slices_bytes(size_t M, size_t N, size_t K, size_t G, bool ragged, const b200_linear_grads &g) {
+    const uint32_t slices = g.dB ? weight_slices(M, N, K, G, ragged) : 1u;
+    return slices > 1 ? align256(slices * N * K * sizeof(float)) : 0;
+}
+
 // Weight form: dB_g = dZ_g^T A_g.
 static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, const int32_t *offsets, size_t M, size_t N, size_t K,
-                      size_t G, const b200_linear_grads &g, bool overlap, cudaStream_t stream) {
+                      size_t G, const b200_linear_grads &g, void *parts, bool overlap, cudaStream_t stream) {
     GroupedParams p;
     memset(&p, 0, sizeof(p));
     p.out = dB;
     p.offsets = offsets;
     p.error_word = st.error_word;
     p.rows = static_cast<uint32_t>(M);
-    p.groups = static_cast<uint32_t>(G);
     p.p_dim = static_cast<uint32_t>(N);
     p.q_dim = static_cast<uint32_t>(K);
     p.in_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
     p.out_type = static_cast<uint32_t>(g.db_type);
     p.accumulate = g.accumulate ? 1u : 0u;
-    const int cg = weight_cg(st, M, N, K, G);
+    size_t longest = M;  // rows of the longest sum there can be
+    const uint32_t slices = weight_slices(M, N, K, G, offsets != nullptr);
+    if (slices > 1) {
+        p.out = parts;
+        p.out_type = B200_C_F32;
+        p.accumulate = 0;
+        p.slice_rows = static_cast<uint32_t>((M + slices - 1) / slices);
+        G = ceil_div_u32(M, p.slice_rows);  // (rounding up may leave the last ones without rows)
+        longest = p.slice_rows;
+    }
+    p.groups = static_cast<uint32_t>(G);
+    const int cg = slices > 1 ? 1 : weight_cg(st, M, N, K, G);
     p.p_blocks = ceil_div_u32(N, 128u * cg);
     p.q_blocks = ceil_div_u32(K, 128u * cg);
     const uint64_t tiles = static_cast<uint64_t>(G) * p.p_blocks * p.q_blocks;
@@ -238,8 +269,29 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
     int rc;
     if ((rc = columns_map(st, dZ, M, N, &p.tm_p, &p.p_wide)) != B200_HGEMM_OK) return rc;
     if ((rc = columns_map(st, A, M, K, &p.tm_q[0], &p.q_wide)) != B200_HGEMM_OK) return rc;
-    const bool f32 = g.db_type == B200_C_F32;
-    if ((rc = get_tensor_map(st, dB, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
+    const bool f32 = p.out_type == B200_C_F32;
+    if ((rc = get_tensor_map(st, p.out, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
+    if (slices > 1) {
+        rc = longest > kLongSum ? launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, overlap, stream)
+                                : launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, overlap, stream);
+        if (rc != B200_HGEMM_OK) return rc;
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cudaLaunchAttribute attrs[2];
+        const size_t count4 = N * K / 4;
+        cfg.gridDim = dim3(ceil_div_u32(count4, 256), 1, 1);
+        cfg.blockDim = dim3(256, 1, 1);
+        cfg.stream = stream;
+        cfg.attrs = attrs;
+        cfg.numAttrs = launch_attributes(attrs, 1, false);
+        if (!cuda_ok(cudaLaunchKernelEx(&cfg, slice_sum_kernel, static_cast<const float4 *>(parts), dB, count4, p.groups,
+                                        static_cast<uint32_t>(g.db_type), g.accumulate ? 1u : 0u),
+                     "cudaLaunchKernelEx")) {
+            return B200_HGEMM_ERR_CUDA;
+        }
+        g_launches.fetch_add(1, std::memory_order_relaxed);
+        return B200_HGEMM_OK;
+    }
     if (f32 && M > kLongSum) {
         if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, overlap, stream);
         return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, overlap, stream);
@@ -267,10 +319,6 @@ static uint32_t slope_slices(size_t M, size_t N, size_t G) {
 // Whether the products read a dZ other than the caller's dC.
 static bool needs_dz(const b200_linear_grads &g) {
     return g.act != B200_ACT_NONE || g.c_type != g.in_type;
-}
-
-static size_t align256(size_t v) {
-    return (v + 255) / 256 * 256;
 }
 
 static size_t dz_bytes(size_t M, size_t N, const b200_linear_grads &g) {
@@ -413,8 +461,9 @@ static int backward(const void *A, const void *B, const int32_t *offsets, size_t
     if (g.accumulate && g.dB && g.db_type != B200_C_F32) return B200_HGEMM_ERR_UNSUPPORTED;
     if (misaligned({A, B, g.dC, g.pre, g.dZ, g.dA, g.dB, g.dbias})) return B200_HGEMM_ERR_MISALIGNED;
     const size_t need_dz = dz_bytes(M, N, g), need_sums = sums_bytes(M, N, G, g);
-    if (need_dz + need_sums > 0) {
-        if (!workspace || workspace_bytes < need_dz + need_sums) return B200_HGEMM_ERR_WORKSPACE;
+    const size_t need_parts = slices_bytes(M, N, K, G, offsets != nullptr, g);
+    if (need_dz + need_sums + need_parts > 0) {
+        if (!workspace || workspace_bytes < need_dz + need_sums + need_parts) return B200_HGEMM_ERR_WORKSPACE;
         if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200_HGEMM_ERR_MISALIGNED;
     }
     DeviceState *st = nullptr;
@@ -447,7 +496,7 @@ static int backward(const void *A, const void *B, const int32_t *offsets, size_t
         passed = false;
         if (rc != B200_HGEMM_OK) return rc;
     }
-    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, !passed, stream);
+    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, ws + need_dz + need_sums, !passed, stream);
     return B200_HGEMM_OK;
 }
 
@@ -477,7 +526,8 @@ int b200_hgemm_linear_backward(const void *A, const void *B, size_t M, size_t N,
 
 size_t b200_hgemm_backward_workspace_bytes(size_t M, size_t N, size_t K, size_t G, const b200_linear_grads *grads) {
     if (!grads || N == 0 || K == 0 || G == 0) return 0;
-    return dz_bytes(M, N, *grads) + sums_bytes(M, N, G, *grads);
+    // (G = 1 may be either form: the dense one's share is counted)
+    return dz_bytes(M, N, *grads) + sums_bytes(M, N, G, *grads) + slices_bytes(M, N, K, G, false, *grads);
 }
 
 }  // extern "C"

@@ -62,7 +62,6 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopePara
     const uint32_t col = blockIdx.x * kSlopeColumns + lane * 8u;
     const uint32_t slice = blockIdx.y, g = blockIdx.z;
     pdl_wait_prior_grids();
-    pdl_launch_dependents();
     uint32_t start = 0, end = p.rows;
     if (p.offsets) {
         const int32_t a = __ldg(p.offsets + g), b = __ldg(p.offsets + g + 1);
@@ -142,6 +141,33 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *sums, float 
 #pragma unroll 8
     for (uint32_t s = 0; s < slices; ++s) total += sums[static_cast<size_t>(s) * count + i];
     dbias[i] = total;
+}
+
+// out[i] = sum of the slices' FP32 results, in order, rounded to out's type (0 FP16, 1 BF16, 2 FP32; added to what is
+// there with `accumulate`, FP32 only). Four values per thread; count is a multiple of 4.
+__global__ void __launch_bounds__(256) slice_sum_kernel(const float4 *slices, void *out, size_t count4, uint32_t n, uint32_t type,
+                                                        uint32_t accumulate) {
+    pdl_wait_prior_grids();
+    const size_t i = static_cast<size_t>(blockIdx.x) * 256u + threadIdx.x;
+    if (i >= count4) return;
+    float4 total = accumulate ? static_cast<const float4 *>(out)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (uint32_t s = 0; s < n; ++s) {
+        const float4 v = slices[static_cast<size_t>(s) * count4 + i];
+        total.x += v.x;
+        total.y += v.y;
+        total.z += v.z;
+        total.w += v.w;
+    }
+    if (type == 2u) {
+        static_cast<float4 *>(out)[i] = total;
+    } else if (type == 1u) {
+        __nv_bfloat162 a = __floats2bfloat162_rn(total.x, total.y), b = __floats2bfloat162_rn(total.z, total.w);
+        static_cast<uint2 *>(out)[i] = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+    } else {
+        __half2 a = __floats2half2_rn(total.x, total.y), b = __floats2half2_rn(total.z, total.w);
+        static_cast<uint2 *>(out)[i] = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+    }
 }
 
 }  // namespace b200

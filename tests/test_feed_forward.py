@@ -231,7 +231,7 @@ def test_linear_residual_in_place_and_no_rows(cuda_device):
 # ------------------------------------------------------------------------------------------------ linear, backward
 BACKWARD_SHAPES = [
     (1, 8, 8), (1, 64, 72), (15, 136, 40), (16, 16, 16), (17, 128, 256), (33, 1024, 64), (64, 72, 1032), (130, 264, 520),
-    (500, 1000, 136), (1000, 2304, 2304), (2049, 256, 128),
+    (500, 1000, 136), (1000, 2304, 2304), (2049, 256, 128), (1024, 1024, 1024), (5000, 72, 200), (8191, 264, 136),
 ]
 
 
