@@ -20,7 +20,8 @@
 // FP32 results of long sums (LONG): the tensor cores cut off what an accumulator cannot hold instead of rounding
 // it, a relative 1.7e-6 after 128 MMAs (a sum of 2048) and growing with the length. That is nothing next to
 // a 16-bit result's rounding, but 30 times FP32's own. Those sums are cut into pieces of kLongBlocks k-blocks that
-// alternate between the two accumulators, and the epilogue warps add the pieces in registers, rounding to nearest.
+// alternate between the two accumulators, and the epilogue warps add the pieces in registers, rounding to nearest
+// (pieces of 1024: 0.8 to 1.0e-6 whatever the length; of 512, as here, half of that).
 //
 // Group sizes are known on the device only (a router wrote them): every CTA reads the offsets, cuts the groups
 // into tiles and walks its share of them. Offsets that are out of order or past T are held within [0, T].

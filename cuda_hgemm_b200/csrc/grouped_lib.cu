@@ -127,7 +127,8 @@ static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_di
             const double tiles = static_cast<double>(blocks * live) * ceil_div_u32(p_dim, 128u * shape.cg);
             const double active = tiles < slots ? tiles : slots;
             double per_block = active * shape.cg * (16384.0 + q / shape.cg * 128.0) / 20.5e6;
-            const double mma = (active * shape.cg > 100.0 ? 0.0013 : 0.0011) * q;
+            // (lower blocks read the weights more often: 6 percent more at none, measured 2 at 205 rows instead of 256)
+            const double mma = (active * shape.cg > 100.0 ? 0.0013 : 0.0011) * q * (1.06 - 0.06 * q / 256.0);
             const double issue = kernel == kRowsSingle128 ? 0.14 : 0.10;
             if (per_block < mma) per_block = mma;
             if (per_block < issue) per_block = issue;
@@ -218,13 +219,15 @@ static int weight_cg(const DeviceState &st, size_t M, size_t N, size_t K, size_t
 
 // Slices a dense layer's long sum over the rows is cut into where its gradient has too few tiles for the GPU: as many as
 // give every SM a tile, of at least 512 rows each. They lie in FP32 in the workspace (20 MB at most) and slice_sum_kernel
-// adds them in order. 8192 rows of 256 x 256: 31 us in one piece, 10 in sixteen.
+// adds them in order. 8192 rows of 256 x 256: 31 us in one piece, 11 in sixteen; of 1024 x
+// 1024: 33 us, 26 in two.
 static uint32_t weight_slices(size_t M, size_t N, size_t K, size_t G, bool ragged) {
     constexpr uint64_t kSms = 148;  // (of a B200; the workspace size must not depend on the current device)
     if (ragged || G != 1 || M < 1024) return 1;
     const uint64_t tiles = static_cast<uint64_t>(ceil_div_u32(N, 128)) * ceil_div_u32(K, 128);
     const uint64_t slices = kSms / tiles < M / 512 ? kSms / tiles : M / 512;
-    return slices < 2 ? 1u : static_cast<uint32_t>(slices);
+    // the sum of the slices is a kernel of its own, about 4 us: 1600 rows' worth of one tile's sum
+    return slices < 2 || M - M / slices < 1600 ? 1u : static_cast<uint32_t>(slices);
 }
 
 static size_t align256(size_t v) {

@@ -85,7 +85,7 @@ int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t col
 bool pdl_enabled();
 
 // Longest sum an FP32 result may take from one accumulator of the tensor cores (gemm_kernel_grouped.cuh says why).
-constexpr uint32_t kLongSum = 1024;
+constexpr uint32_t kLongSum = 512;
 // A linear layer on the grouped kernel, all rows one group (arguments checked by the caller).
 int run_linear_rows(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args &args,
                     cudaStream_t stream);

@@ -137,7 +137,8 @@ def check_backward(dC, A, B, act, pre, dZ, dA, dB, dbias, what, dB_was=None, dbi
 # ------------------------------------------------------------------------------------------------ linear, forward
 LINEAR_SHAPES = [
     (1, 8, 8), (1, 64, 72), (3, 1, 16), (16, 1024, 512), (17, 33, 40), (64, 4099, 136), (16, 4096, 4096), (100, 512, 4096),
-    (128, 4096, 1024), (128, 4096, 8192), (40, 1024, 4096), (129, 257, 64), (300, 700, 200), (777, 1000, 520), (1024, 2048, 256),
+    (128, 4096, 1024), (128, 4096, 8192), (40, 1024, 4096), (129, 257, 64), (300, 700, 200), (777, 1000, 520), (1024, 2048, 256), (200, 4096, 4096),
+    (777, 4099, 2056),
 ]
 
 
@@ -185,15 +186,16 @@ def test_linear_forward_large_tiles(cuda_device, dtype, act, with_pre):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_fp32_results_of_long_sums(cuda_device, dtype):
-    """The tensor cores cut an accumulator off at every MMA, on average by half of 2^-23 of it: a sum of 1024 (64 MMAs)
-    is off by at most 64 * 2^-24 in the mean, and so is a longer one, whose pieces are added in FP32 (rounding to
-    nearest adds 2^-24 each, at random). One accumulator for all of a sum of 16384 would be off by sixteen times that."""
+    """The tensor cores cut an accumulator off at every MMA, on average by half of 2^-23 of it: a sum of 512 (32 MMAs)
+    is off by at most 32 * 2^-24 in the mean, and so is a longer one, whose pieces are added in FP32 (rounding to
+    nearest adds at most 2^-24 each, a quarter of it in the mean). One accumulator for all of a sum of 16384 would be
+    off by 32 times that."""
     import torch
 
     from cuda_hgemm_b200 import api
 
-    limit = 64 * 2.0 ** -24 + 16 * 2.0 ** -24 / 4
-    for M, N, K in ((16, 264, 16384), (200, 264, 16384), (2000, 2568, 16384)):
+    limit = 32 * 2.0 ** -24 + 32 * 2.0 ** -24 / 4
+    for M, N, K in ((16, 264, 16384), (200, 264, 16384), (512, 4096, 16384), (2000, 2568, 16384)):
         A, B = make((M, K), dtype, cuda_device, 1), make((N, K), dtype, cuda_device, 2)
         C = torch.empty((M, N), device=cuda_device)
         api.hgemm_linear(A, B, C)
@@ -232,6 +234,7 @@ def test_linear_residual_in_place_and_no_rows(cuda_device):
 BACKWARD_SHAPES = [
     (1, 8, 8), (1, 64, 72), (15, 136, 40), (16, 16, 16), (17, 128, 256), (33, 1024, 64), (64, 72, 1032), (130, 264, 520),
     (500, 1000, 136), (1000, 2304, 2304), (2049, 256, 128), (1024, 1024, 1024), (5000, 72, 200), (8191, 264, 136),
+    (300, 4096, 2048), (1333, 4104, 2040),
 ]
 
 
@@ -360,8 +363,7 @@ def test_grouped_forward_on_pairs(cuda_device, dtype, out, act):
     """Enough tiles for the pair kernel: several blocks of rows per group, a stack with gaps, a ragged last block."""
     sizes = [400, 37, 0, 1031, 256, 300, 511, 222]
     forward_of_groups(cuda_device, sizes, 1416, 328, dtype, out, act, True, act != "none", gap=8)
-    if out == F32:  # a long sum, added up in pieces
-        forward_of_groups(cuda_device, sizes, 1416, 2184, dtype, out, act, True, False)
+    forward_of_groups(cuda_device, sizes, 1416, 2184, dtype, out, act, True, act != "none")  # (FP32: added up in pieces)
 
 
 def backward_of_groups(device, sizes, N, K, dtype, out, act, db_type, gap=0, accumulate=False):
@@ -415,13 +417,22 @@ def test_grouped_backward_on_pairs(cuda_device, shape, dtype, db_type):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,db_type", [(F16, F16), (BF16, F32)])
+def test_grouped_backward_of_long_groups(cuda_device, dtype, db_type):
+    """Groups long enough for pairs in the weights' gradient too, most of them ending inside a block of 64 rows."""
+    sizes = [2600, 37, 0, 4031, 777, 3000]
+    backward_of_groups(cuda_device, sizes, 2040, 1528, dtype, dtype, "silu", db_type)
+    backward_of_groups(cuda_device, sizes, 2048, 1536, dtype, dtype, "none", F32, accumulate=True)
+
+
+@pytest.mark.gpu
 def test_rows_of_the_next_group_stay_out_of_a_weight_gradient(cuda_device):
     """A NaN in one group's rows makes its own gradients NaN and nobody else's."""
     import torch
 
     from cuda_hgemm_b200 import api
 
-    for N, K, sizes in ((136, 72, [5, 7, 70, 64, 3]), (1032, 1032, [5, 7, 70, 64, 3, 129, 1])):  # single CTAs, pairs
+    for N, K, sizes in ((136, 72, [5, 7, 70, 64, 3]), (2040, 1528, [1000, 7, 2070, 640, 3, 1290, 1])):  # single CTAs, pairs
         M, bounds, offsets, A, B = group_inputs(sizes, N, K, F16, cuda_device)
         dC = make((M, N), F16, cuda_device, 5)
         bad = 1
@@ -455,6 +466,36 @@ def test_offsets_out_of_order_stay_inside_the_operands(cuda_device):
         api.hgemm_grouped_backward(C, A, B, offsets, dA=dA, dB=dB, act="silu", pre=C)
         assert (room[M:] == SENTINEL).all()
     check_forward(A, B[3], None, None, "none", room[:M], None, "last group")
+    assert api.last_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_the_32_elements(cuda_device):
+    """An output of 4.6e9 elements: its last rows lie beyond what 32 bits count."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    M, N, K = 70001, 65536, 8
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("not enough free memory")
+    A, B = make((M, K), BF16, cuda_device, 1), make((N, K), BF16, cuda_device, 2)
+    bias = make((N,), BF16, cuda_device, 3)
+    C = torch.empty((M, N), dtype=torch.bfloat16, device=cuda_device)
+    api.hgemm_linear(A, B, C, bias=bias, act="gelu")
+    for rows in (slice(0, 3), slice(65534, 65539), slice(M - 3, M)):
+        check_forward(A[rows], B, bias, None, "gelu", C[rows], None, str(rows))
+    dA, dbias = torch.empty_like(A), torch.empty(N, device=cuda_device)
+    dB = torch.empty((N, K), device=cuda_device)
+    C[:M - 2] = 0  # what is left to sum lies in the last two rows
+    api.hgemm_linear_backward(C, A, B, dA=dA, dB=dB, dbias=dbias)
+    last = slice(M - 2, M)
+    check_backward(C[last], A[last], B, "none", None, None, dA[last], dB, dbias, "last rows")
+    assert (dA[:M - 2] == 0).all()
+    offsets = torch.tensor([0, 5, M], dtype=torch.int32, device=cuda_device)
+    C.fill_(SENTINEL)
+    api.hgemm_grouped(A, torch.stack([B, B.flip(0)]), C, offsets, act="relu")
+    check_forward(A[last], B.flip(0), None, None, "relu", C[last], None, "last group")
     assert api.last_device_error() == 0
 
 
