@@ -32,7 +32,8 @@
 // overwritten with zeros in both operands before the MMA reads them, so that whatever the next group holds, NaN
 // included, stays out of the sum.
 //
-// Warp roles, ring, accumulators and bounded waits are those of hgemm_tcgen05_kernel (gemm_kernel.cuh); the
+// Warp roles, ring, accumulators and bounded waits are those of hgemm_tcgen05_kernel (gemm_kernel.cuh); unlike there
+// neither this kernel nor its successor starts early (grouped_lib.cu says why). The
 // reference has no counterpart (one product per launch, src/main.cu:11).
 #pragma once
 
@@ -378,7 +379,6 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
         tmem_alloc<CG>(smem_u32(const_cast<uint32_t *>(tmem_slot)), T::kTmemCols);
         tmem_relinquish<CG>();
     }
-    pdl_wait_prior_grids();  // offsets and operands may have been written, and outputs read, by the previous kernel
 
     uint32_t tiles;
     if (WEIGHT) {
@@ -415,8 +415,6 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
     if (CG == 2) cluster_sync_all();  // the peer's copies and arrivals target this CTA's barriers
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
-    // Only now, with the kernel before this one complete: no more than two kernels of a chain are ever on the GPU.
-    pdl_launch_dependents();
     // Columns of the result per tile. Where a tile takes few rows its time is that of reading its weights, and the
     // kernel's that of the SM with the most of them: 26 groups of 1024 columns are 208 tiles of 128, two for an SM, or 286 of
     // 96, two for an SM as well. The width with the least waves x (width + the rows' share of a stage and a tile's fixed

@@ -27,41 +27,31 @@ static bool misaligned(std::initializer_list<const void *> ptrs) {
     return (bits & 15u) != 0;
 }
 
-// Kernel attributes of one launch: programmatic dependent launch where `overlap` allows it, and the pair where there is
-// one. The pass over dC starts behind the kernel before it, and a product behind that pass, without overlap: the
-// small CTAs of the one and the whole-SM pairs of the other, started early and waiting beside each other, have
-// been seen to stand still for good. Between two products the overlap stays.
-static int launch_attributes(cudaLaunchAttribute *attrs, int cg, bool overlap) {
-    int n = 0;
-    if (overlap && pdl_enabled()) {
-        attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
-    if (cg == 2) {
-        attrs[n].id = cudaLaunchAttributeClusterDimension;
-        attrs[n].val.clusterDim.x = 2;
-        attrs[n].val.clusterDim.y = 1;
-        attrs[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    return n;
+// All kernels here are launched plainly, each when the one before it in the stream has ended. Started early
+// (programmatic dependent launch, 1 to 2 us less between two of them) and waiting beside one another, the small
+// CTAs of the pass over dC and the whole-SM CTAs and pairs of the products have been seen to stand still for good.
+static void pair_attribute(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr) {
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = 2;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
 }
 
 // `most_tiles`: an upper bound of the tiles there can be; the grid is persistent and never larger than what
 // is resident at once.
 template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG = false>
-static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uint64_t most_tiles, bool overlap, cudaStream_t stream) {
+static int launch_grouped(DeviceState &st, int slot, const GroupedParams &p, uint64_t most_tiles, cudaStream_t stream) {
     using T = GroupedTraits<FORM, CG, QT, STAGES, KPS, LONG>;
     auto kern = hgemm_grouped_kernel<FORM, CG, QT, STAGES, KPS, LONG>;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute attrs[2];
+    cudaLaunchAttribute attr;
     cfg.blockDim = dim3(kGroupedThreads, 1, 1);
     cfg.dynamicSmemBytes = T::kSmemBytes;
     cfg.stream = stream;
-    cfg.attrs = attrs;
-    cfg.numAttrs = launch_attributes(attrs, CG, overlap);
+    if (CG == 2) pair_attribute(&cfg, &attr);
     uint32_t resident = static_cast<uint32_t>(st.sm_count);
     {
         std::lock_guard<std::mutex> lock(st.mu);
@@ -145,7 +135,7 @@ static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_di
 // Forward and input form. X: the rows' operand [rows x k_dim]; W: groups matrices [w_rows x w_cols], stride_w apart.
 template <int FORM>
 static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, size_t p_dim, size_t k_dim, size_t w_rows,
-                    size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, bool overlap, cudaStream_t stream) {
+                    size_t w_cols, size_t groups, size_t stride_w, GroupedParams &p, cudaStream_t stream) {
     constexpr int kSlots = FORM == kFormForward ? 96 : 104;
     p.error_word = st.error_word;
     p.rows = static_cast<uint32_t>(rows);
@@ -175,18 +165,18 @@ static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, 
     if constexpr (FORM == kFormForward) {
         if (p.out_type == B200_C_F32 && k_dim > kLongSum) {
             switch (plan.kernel) {
-                case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, overlap, stream);
-                case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, overlap, stream);
-                case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, overlap, stream);
-                default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, overlap, stream);
+                case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, stream);
+                case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, stream);
+                case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, stream);
+                default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, stream);
             }
         }
     }
     switch (plan.kernel) {
-        case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1>(st, slot, p, tiles, overlap, stream);
-        case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2>(st, slot, p, tiles, overlap, stream);
-        case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2>(st, slot, p, tiles, overlap, stream);
-        default: return launch_grouped<FORM, 1, 32, 5, 2>(st, slot, p, tiles, overlap, stream);
+        case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1>(st, slot, p, tiles, stream);
+        case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2>(st, slot, p, tiles, stream);
+        case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2>(st, slot, p, tiles, stream);
+        default: return launch_grouped<FORM, 1, 32, 5, 2>(st, slot, p, tiles, stream);
     }
 }
 
@@ -241,7 +231,7 @@ static size_t slices_bytes(size_t M, size_t N, size_t K, size_t G, bool ragged, 
 
 // Weight form: dB_g = dZ_g^T A_g.
 static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, const int32_t *offsets, size_t M, size_t N, size_t K,
-                      size_t G, const b200_linear_grads &g, void *parts, bool overlap, cudaStream_t stream) {
+                      size_t G, const b200_linear_grads &g, void *parts, cudaStream_t stream) {
     GroupedParams p;
     memset(&p, 0, sizeof(p));
     p.out = dB;
@@ -275,18 +265,15 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
     const bool f32 = p.out_type == B200_C_F32;
     if ((rc = get_tensor_map(st, p.out, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
     if (slices > 1) {
-        rc = longest > kLongSum ? launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, overlap, stream)
-                                : launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, overlap, stream);
+        rc = longest > kLongSum ? launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, stream)
+                                : launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, stream);
         if (rc != B200_HGEMM_OK) return rc;
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
-        cudaLaunchAttribute attrs[2];
-        const size_t count4 = N * K / 4;
+            const size_t count4 = N * K / 4;
         cfg.gridDim = dim3(ceil_div_u32(count4, 256), 1, 1);
         cfg.blockDim = dim3(256, 1, 1);
         cfg.stream = stream;
-        cfg.attrs = attrs;
-        cfg.numAttrs = launch_attributes(attrs, 1, false);
         if (!cuda_ok(cudaLaunchKernelEx(&cfg, slice_sum_kernel, static_cast<const float4 *>(parts), dB, count4, p.groups,
                                         static_cast<uint32_t>(g.db_type), g.accumulate ? 1u : 0u),
                      "cudaLaunchKernelEx")) {
@@ -296,11 +283,11 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
         return B200_HGEMM_OK;
     }
     if (f32 && M > kLongSum) {
-        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, overlap, stream);
-        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, overlap, stream);
+        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, stream);
+        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, stream);
     }
-    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 110, p, tiles, overlap, stream);
-    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, overlap, stream);
+    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 110, p, tiles, stream);
+    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, stream);
 }
 
 // ---- the pass over dC -----------------------------------------------------------------------
@@ -347,12 +334,9 @@ static cudaError_t launch_slope_kernel(const cudaLaunchConfig_t *cfg, const Slop
 static int launch_slope(const SlopeParams &p, uint32_t act, dim3 grid, cudaStream_t stream) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute attrs[2];
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kSlopeThreads, 1, 1);
     cfg.stream = stream;
-    cfg.attrs = attrs;
-    cfg.numAttrs = launch_attributes(attrs, 1, false);
     const cudaError_t e = p.c_type == B200_C_F32 ? launch_slope_kernel<true>(&cfg, p, act) : launch_slope_kernel<false>(&cfg, p, act);
     if (!cuda_ok(e, "cudaLaunchKernelEx")) return B200_HGEMM_ERR_CUDA;
     g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -381,13 +365,10 @@ static int run_slope(const b200_linear_grads &g, void *dz, float *sums, const in
     if (rc != B200_HGEMM_OK || !g.dbias || one) return rc;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute attrs[2];
     const size_t count = G * N;
     cfg.gridDim = dim3(ceil_div_u32(count, 256), 1, 1);
     cfg.blockDim = dim3(256, 1, 1);
     cfg.stream = stream;
-    cfg.attrs = attrs;
-    cfg.numAttrs = launch_attributes(attrs, 1, true);
     if (!cuda_ok(cudaLaunchKernelEx(&cfg, bias_sum_kernel, static_cast<const float *>(sums), g.dbias, count, p.slices,
                                     g.accumulate ? 1u : 0u),
                  "cudaLaunchKernelEx")) {
@@ -428,7 +409,7 @@ static GroupedParams forward_params(void *C, const int32_t *offsets, const b200_
 int run_linear_rows(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args &args,
                     cudaStream_t stream) {
     GroupedParams p = forward_params(C, nullptr, args);
-    return run_rows<kFormForward>(st, A, B, M, N, K, N, K, 1, N * K, p, true, stream);
+    return run_rows<kFormForward>(st, A, B, M, N, K, N, K, 1, N * K, p, stream);
 }
 
 static int grouped_forward(const void *A, const void *B, void *C, const int32_t *offsets, size_t M, size_t N, size_t K, size_t G,
@@ -445,7 +426,7 @@ static int grouped_forward(const void *A, const void *B, void *C, const int32_t 
     if ((rc = current_state(&st)) != B200_HGEMM_OK) return rc;
     if (!st->sm100) return B200_HGEMM_ERR_NO_SM100;
     GroupedParams p = forward_params(C, offsets, *args);
-    return run_rows<kFormForward>(*st, A, B, M, N, K, N, K, G, G > 1 ? stride_b : N * K, p, true, stream);
+    return run_rows<kFormForward>(*st, A, B, M, N, K, N, K, G, G > 1 ? stride_b : N * K, p, stream);
 }
 
 // Both backward entry points; `offsets` is null for the dense one.
@@ -483,8 +464,7 @@ static int backward(const void *A, const void *B, const int32_t *offsets, size_t
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     void *dz = g.dZ ? g.dZ : (need_dz ? ws : nullptr);
     float *sums = reinterpret_cast<float *>(ws + need_dz);
-    bool passed = dz || g.dbias;  // the next product follows the pass over dC
-    if (passed) {
+    if (dz || g.dbias) {
         if ((rc = run_slope(g, dz, sums, offsets, M, N, G, stream)) != B200_HGEMM_OK) return rc;
     }
     const void *dz_read = needs_dz(g) ? dz : g.dC;
@@ -495,11 +475,10 @@ static int backward(const void *A, const void *B, const int32_t *offsets, size_t
         p.offsets = offsets;
         p.in_bf16 = g.in_type == B200_C_BF16 ? 1u : 0u;
         p.out_type = static_cast<uint32_t>(g.in_type);
-        rc = run_rows<kFormInput>(*st, dz_read, B, M, K, N, N, K, G, G > 1 ? stride_b : N * K, p, !passed, stream);
-        passed = false;
+        rc = run_rows<kFormInput>(*st, dz_read, B, M, K, N, N, K, G, G > 1 ? stride_b : N * K, p, stream);
         if (rc != B200_HGEMM_OK) return rc;
     }
-    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, ws + need_dz + need_sums, !passed, stream);
+    if (g.dB) return run_weight(*st, dz_read, A, g.dB, offsets, M, N, K, G, g, ws + need_dz + need_sums, stream);
     return B200_HGEMM_OK;
 }
 

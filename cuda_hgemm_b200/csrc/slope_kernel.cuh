@@ -61,7 +61,6 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopePara
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t col = blockIdx.x * kSlopeColumns + lane * 8u;
     const uint32_t slice = blockIdx.y, g = blockIdx.z;
-    pdl_wait_prior_grids();
     uint32_t start = 0, end = p.rows;
     if (p.offsets) {
         const int32_t a = __ldg(p.offsets + g), b = __ldg(p.offsets + g + 1);
@@ -134,7 +133,6 @@ __global__ void __launch_bounds__(kSlopeThreads, 4) slope_kernel(const SlopePara
 
 // dbias[i] = sum of the slices' sums, in order (added to what is there with `accumulate`).
 __global__ void __launch_bounds__(256) bias_sum_kernel(const float *sums, float *dbias, size_t count, uint32_t slices, uint32_t accumulate) {
-    pdl_wait_prior_grids();
     const size_t i = static_cast<size_t>(blockIdx.x) * 256u + threadIdx.x;
     if (i >= count) return;
     float total = accumulate ? dbias[i] : 0.f;
@@ -147,7 +145,6 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *sums, float 
 // there with `accumulate`, FP32 only). Four values per thread; count is a multiple of 4.
 __global__ void __launch_bounds__(256) slice_sum_kernel(const float4 *slices, void *out, size_t count4, uint32_t n, uint32_t type,
                                                         uint32_t accumulate) {
-    pdl_wait_prior_grids();
     const size_t i = static_cast<size_t>(blockIdx.x) * 256u + threadIdx.x;
     if (i >= count4) return;
     float4 total = accumulate ? static_cast<const float4 *>(out)[i] : make_float4(0.f, 0.f, 0.f, 0.f);

@@ -591,6 +591,50 @@ def test_captured_replayed_and_on_another_stream(cuda_device):
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once(cuda_device):
+    """Forward and backward calls of two layers, each on its own stream, run into each other: the bits of a run alone."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    layers = []
+    for seed, (sizes, N, K) in enumerate((([300, 0, 5, 700], 520, 264), ([64, 900, 33], 1032, 520))):
+        M, bounds, offsets, A, B = group_inputs(sizes, N, K, BF16, cuda_device)
+        G = len(sizes)
+        layers.append(dict(A=A, B=B, offsets=offsets, dC=make((M, N), BF16, cuda_device, 50 + seed), G=G, N=N, K=K, M=M))
+
+    def outputs(l):
+        new = lambda shape, dt: torch.zeros(shape, dtype=dt, device=cuda_device)  # noqa: E731
+        return dict(C=new((l["M"], l["N"]), torch.bfloat16), pre=new((l["M"], l["N"]), torch.bfloat16), dA=new((l["M"], l["K"]), torch.bfloat16),
+                    dB=new((l["G"], l["N"], l["K"]), torch.float32), dbias=new((l["G"], l["N"]), torch.float32),
+                    D=new((16, l["N"]), torch.bfloat16))
+
+    def step(l, o):
+        api.hgemm_grouped(l["A"], l["B"], o["C"], l["offsets"], act="gelu", pre=o["pre"])
+        api.hgemm_linear(l["A"][8:24], l["B"][0], o["D"], act="silu")
+        api.hgemm_grouped_backward(l["dC"], l["A"], l["B"], l["offsets"], act="gelu", pre=o["pre"], dA=o["dA"], dB=o["dB"], dbias=o["dbias"])
+
+    alone = []
+    for l in layers:
+        o = outputs(l)
+        step(l, o)
+        torch.cuda.synchronize()
+        alone.append(o)
+    streams = [torch.cuda.Stream() for _ in layers]
+    together = [outputs(l) for l in layers]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for l, o, s in zip(layers, together, streams):
+            with torch.cuda.stream(s):
+                step(l, o)
+    torch.cuda.synchronize()
+    for a, b in zip(alone, together):
+        for name in a:
+            assert torch.equal(a[name], b[name]), name
+    assert api.last_device_error() == 0
+
+
+@pytest.mark.gpu
 def test_same_inputs_same_bits(cuda_device):
     import torch
 
