@@ -202,7 +202,7 @@ def _operand(name, t, dtypes, shape, device):
     absent one)."""
     if t is None:
         return None
-    if getattr(t, "dtype", None) not in dtypes or not t.is_cuda or not t.is_contiguous():
+    if getattr(t, "dtype", None) not in dtypes or not t.is_cuda or not t.is_contiguous():  # (also what is no tensor at all)
         raise TypeError(f"{name} must be a contiguous CUDA tensor of type {' or '.join(str(d)[6:] for d in dtypes)}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
@@ -216,19 +216,22 @@ def _rows_and_weights(A, B, offsets):
     import torch
 
     grouped = offsets is not None
-    for name, t, dims in (("A", A, 2), ("B", B, 3 if grouped else 2)):
-        if getattr(t, "dtype", None) not in (torch.float16, torch.bfloat16) or not t.is_cuda:
-            raise TypeError(f"{name} must be a float16 or bfloat16 CUDA tensor")
-        if t.dim() != dims:
-            raise ValueError(f"{name} must be {dims}-D")
-    if A.dtype != B.dtype:
-        raise TypeError("A and B must have one type")
+    dtype = getattr(A, "dtype", None)
+    if (dtype is not torch.float16 and dtype is not torch.bfloat16) or not A.is_cuda:
+        raise TypeError("A must be a float16 or bfloat16 CUDA tensor")
+    if getattr(B, "dtype", None) is not dtype or not B.is_cuda:
+        raise TypeError("B must be a CUDA tensor of A's type")
+    a_shape, b_shape = A.shape, B.shape
+    if len(a_shape) != 2:
+        raise ValueError("A must be 2-D")
+    if len(b_shape) != (3 if grouped else 2):
+        raise ValueError(f"B must be {3 if grouped else 2}-D")
     if A.get_device() != B.get_device():
         raise ValueError("A and B must live on one device")
-    M, K = A.shape
-    N = B.shape[-2]
-    if B.shape[-1] != K:
-        raise ValueError(f"shape mismatch: A {tuple(A.shape)}, B {tuple(B.shape)}")
+    M, K = a_shape
+    N = b_shape[-2]
+    if b_shape[-1] != K:
+        raise ValueError(f"shape mismatch: A {tuple(a_shape)}, B {tuple(b_shape)}")
     if not A.is_contiguous():
         raise TypeError("A must be contiguous")
     if not grouped:
@@ -273,8 +276,10 @@ def _linear_args(A, C, bias, act, residual, pre, bias_shape, M, N):
     if c_ptr is None:
         raise TypeError("C must be a CUDA tensor")
     return c_ptr, _native.LinearArgs(
-        _type_code(dtype), _type_code(C.dtype), _act_code(act), _operand("bias", bias, (dtype,), bias_shape, device),
-        _operand("residual", residual, (C.dtype,), (M, N), device), _operand("pre", pre, (C.dtype,), (M, N), device))
+        _type_code(dtype), _type_code(C.dtype), _act_code(act),
+        None if bias is None else _operand("bias", bias, (dtype,), bias_shape, device),
+        None if residual is None else _operand("residual", residual, (C.dtype,), (M, N), device),
+        None if pre is None else _operand("pre", pre, (C.dtype,), (M, N), device))
 
 
 def hgemm_linear(A, B, C, bias=None, act: str = "none", residual=None, pre=None):

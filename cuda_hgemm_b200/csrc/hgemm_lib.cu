@@ -114,7 +114,7 @@ int current_state(DeviceState **out) {
 // A 2-D tensor (16-bit elements, or FP32 with elem_bytes = 4) of `rows` x `cols` (cols contiguous) viewed through boxes of
 // box_rows x box_cols, with the 128-byte swizzle (box_cols = 64) or, for plain row-major staging
 // tiles, without. Out-of-range elements read as zero and are dropped on store. The cache is 4-way
-// set-associative (64 sets): a handful of operands in rotation never evict each other.
+// set-associative (256 sets): a handful of operands in rotation never evict each other.
 int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
                    CUtensorMap *out, bool swizzle, uint64_t batch, uint64_t batch_stride, uint32_t elem_bytes,
                    uint64_t pitch, uint32_t box_batch) {
@@ -123,7 +123,9 @@ int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t col
     size_t h = (reinterpret_cast<uintptr_t>(ptr) >> 8) * 0x9E3779B97F4A7C15ull;
     h ^= rows * 0xC2B2AE3D27D4EB4Full + cols * 0x165667B19E3779F9ull + box_rows * 131u + box_cols + (swizzle ? 0u : 77u) +
          batch * 0x9E3779B1ull + batch_stride * 0x85EBCA77ull + elem_bytes + pitch * 0x27D4EB2Full;
-    const size_t set = ((h >> 20) & 63u) * kTensorMapWays;
+    // one operand of the grouped kernels has up to eight maps that differ in the box's height alone: spread them too
+    h ^= static_cast<uint64_t>(box_rows) * 0xD6E8FEB86659FD93ull;
+    const size_t set = ((h >> 20) & (kTensorMapSets - 1)) * kTensorMapWays;
     std::lock_guard<std::mutex> lock(st.mu);
     TensorMapSlot *slot = nullptr;
     for (size_t w = 0; w < kTensorMapWays; ++w) {
@@ -1836,8 +1838,8 @@ int b200_hgemm_fused_ex(const void *A, const void *B, void *C, size_t M, size_t 
 
 // ---- linear layers --------------------------------------------------------------------------------
 // Whether a linear layer runs on the short-A kernels, with which plan. They take batches of up to 64 rows against
-// enough columns to fill the GPU, and batches of up to 128 rows whose long k is cut into ranges (the grouped kernel does not cut
-// it). Everything else runs on the grouped kernel as a single group (run_linear_rows), whose epilogue keeps up with an
+// enough columns to fill the GPU, batches of up to 128 rows whose long k is cut into ranges (the grouped kernel does not cut
+// it), and any k cut for up to 16 rows (1 x 1024 x 1024: 6.5 us against 8.2). Everything else runs on the grouped kernel as a single group (run_linear_rows), whose epilogue keeps up with an
 // activation and with Z beside C. In BF16 with silu, short-A against grouped: 33 x 14336 x 4096 24.8 and 26.3 us, 64
 // rows 23.8 and 25.3, 128 rows 36.2 and 28.7; 64 x 4096 x 14336 26.4 and 35.3; 100 x 2048 x 1024 13.7 and 7.0, 64 x 1024 x 1024
 // 10.3 and 6.7; and 8192 x 14336 x 4096 with gelu and Z 1453 us on the whole-tile kernels with their fused epilogue
@@ -1849,7 +1851,7 @@ static bool linear_plan(const DeviceState &st, size_t M, size_t N, size_t K, con
     select_plan(st, M, N, K, pl);
     if (pl->variant != B200_VARIANT_SKINNY && pl->variant != B200_VARIANT_SKINNY_PAIR) return false;
     const uint32_t slices = skinny_slices(*pl, st, N, K);
-    if (slices == 1 ? M > 64 : K < 4096) return false;
+    if (slices == 1 ? M > 64 : M > 16 && K < 4096) return false;
     if (args.c_type == B200_C_F32 && K > kLongSum * slices) return false;
     if (pl->grid == 0 && skinny_sums_on_chip(*pl, slices) == 1) pl->grid = 1;
     return true;

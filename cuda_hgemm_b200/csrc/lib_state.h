@@ -38,7 +38,7 @@ struct TensorMapSlot {
     TensorMapKey key{};
     CUtensorMap map{};
 };
-constexpr size_t kTensorMapWays = 4;
+constexpr size_t kTensorMapWays = 4, kTensorMapSets = 256;
 
 struct DeviceState {
     std::mutex mu;
@@ -68,7 +68,7 @@ struct DeviceState {
     bool attr_set[128] = {};    // slots from 96 on: the grouped kernels
     int max_clusters[128] = {};
     int ck_clusters[16][9] = {};  // short-A kernels that sum inside clusters: clusters of each size the device holds at once (-1: none)  // CTA pairs the device can keep resident at once, per pair kernel
-    TensorMapSlot tm_cache[64 * kTensorMapWays];
+    TensorMapSlot tm_cache[kTensorMapSets * kTensorMapWays];
     uint64_t tm_clock = 0;
 };
 
