@@ -8,7 +8,7 @@
 //
 // (0.5 (1 + tanh(w/2)) is that s: one exponential and one division instead of a tanh.) A NaN stays a NaN.
 // Where s (1-s) has underflown, z is held at a bound before it multiplies it, so that a large z gives the
-// slope 0 or 1 and not 0 * infinity.
+// slope 0 or 1 and not 0 * infinity. The value at +infinity is +infinity; at -infinity relu gives 0, the others z * 0 = NaN.
 #pragma once
 
 #include <stdint.h>
@@ -54,9 +54,13 @@ __device__ __forceinline__ float normal_tail(float z, float *gauss) {
     return 0.5f * poly * t * *gauss;
 }
 
-// 1 / (1 + exp(-z (a + b z^2))): silu's gate with a = 1, b = 0, that of gelu_tanh with the two constants above.
-__device__ __forceinline__ float logistic_gate(float z, float a, float b) {
-    return __fdividef(1.f, 1.f + exp2_approx(-kLog2e * z * fmaf(b * z, z, a)));
+// 1 / (1 + exp(-w)): the gate of silu (w = z) and of gelu_tanh. Each has its own arithmetic: silu as the other with
+// the cubic's constant 0 would multiply an infinite z by that 0.
+template <uint32_t KIND>
+__device__ __forceinline__ float logistic_gate(float z) {
+    float w = z;
+    if (KIND == kActGeluTanh) w *= fmaf(kGeluTanhScale * kGeluTanhCubic * z, z, kGeluTanhScale);
+    return __fdividef(1.f, 1.f + exp2_approx(-kLog2e * w));
 }
 
 template <uint32_t KIND>
@@ -67,8 +71,7 @@ __device__ __forceinline__ float act_value(float z) {
         const float tail = normal_tail(z, &gauss);
         return z * (z < 0.f ? tail : 1.f - tail);
     }
-    if (KIND == kActGeluTanh) return z * logistic_gate(z, kGeluTanhScale, kGeluTanhScale * kGeluTanhCubic);
-    if (KIND == kActSilu) return z * logistic_gate(z, 1.f, 0.f);
+    if (KIND == kActGeluTanh || KIND == kActSilu) return z * logistic_gate<KIND>(z);
     return z;
 }
 
@@ -83,12 +86,12 @@ __device__ __forceinline__ float act_slope(float z) {
     }
     if (KIND == kActGeluTanh) {
         const float h = held(z, 16.f);
-        const float s = logistic_gate(h, kGeluTanhScale, kGeluTanhScale * kGeluTanhCubic);
+        const float s = logistic_gate<KIND>(h);
         return s + h * s * (1.f - s) * kGeluTanhScale * fmaf(3.f * kGeluTanhCubic * h, h, 1.f);
     }
     if (KIND == kActSilu) {
-        const float h = held(z, 80.f);  // exp(80) is still finite
-        const float s = logistic_gate(h, 1.f, 0.f);
+        const float h = held(z, 88.f);  // exp(88) is still finite, and its reciprocal already 0 (__fdividef, above 2^126)
+        const float s = logistic_gate<KIND>(h);
         return s + h * s * (1.f - s);
     }
     return 1.f;
@@ -103,14 +106,10 @@ __device__ __forceinline__ void act_apply_kind(uint32_t *vals) {
 
 template <int COUNT>
 __device__ __forceinline__ void act_apply(uint32_t *vals, uint32_t kind) {
-    if (kind == kActGeluTanh || kind == kActSilu) {
-        // one loop for both: the gates differ in two constants
-        const float a = kind == kActSilu ? 1.f : kGeluTanhScale, b = kind == kActSilu ? 0.f : kGeluTanhScale * kGeluTanhCubic;
-#pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const float z = __uint_as_float(vals[j]);
-            vals[j] = __float_as_uint(z * logistic_gate(z, a, b));
-        }
+    if (kind == kActGeluTanh) {
+        act_apply_kind<COUNT, kActGeluTanh>(vals);
+    } else if (kind == kActSilu) {
+        act_apply_kind<COUNT, kActSilu>(vals);
     } else if (kind == kActGelu) {
         act_apply_kind<COUNT, kActGelu>(vals);
     } else if (kind == kActRelu) {
