@@ -40,18 +40,23 @@ __device__ __forceinline__ float held(float z, float bound) {
     return z > bound ? bound : (z < -bound ? -bound : z);
 }
 
-// 1 - Phi(|z|) and exp(-z^2/2): erfc(x) = t (a1 + t (a2 + ... a5)) exp(-x^2) with t = 1/(1 + p x), x = |z|/sqrt 2
-// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: absolute error below 1.5e-7, so Phi is off by
-// less than 1e-7). No branch, and about half the instructions of erff, which the epilogue warps would feel.
+// 1 - Phi(|z|) and exp(-z^2/2). The tail is exp(-z^2/2) times a function that falls off like 1/|z|, and that function
+// is a polynomial in t = 1/(1 + 0.3 |z|): the form of Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, with
+// eight terms instead of five, whose coefficients minimise the largest RELATIVE error for |z| <= 13.2 (1.2e-7, found by linear
+// programming in 64 bits; the five-term form is good to 1.5e-7 absolute, which at z = -3 is 5e-5 of gelu's value).
+// In FP32 the result is off by at most 1e-6 relative plus six roundings of z^2/2 (the exponential's argument).
+// No branch, and fewer instructions than erff, which the epilogue warps would feel.
 __device__ __forceinline__ float normal_tail(float z, float *gauss) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    float poly = fmaf(1.061405429f, t, -1.453152027f);
-    poly = fmaf(poly, t, 1.421413741f);
-    poly = fmaf(poly, t, -0.284496736f);
-    poly = fmaf(poly, t, 0.254829592f);
-    *gauss = exp2_approx(-kLog2e * x * x);
-    return 0.5f * poly * t * *gauss;
+    const float t = __fdividef(1.f, fmaf(0.3f, fabsf(z), 1.f));
+    float poly = fmaf(0.0360886529f, t, -0.158932984f);
+    poly = fmaf(poly, t, 0.209345162f);
+    poly = fmaf(poly, t, -0.0564490594f);
+    poly = fmaf(poly, t, 0.130032122f);
+    poly = fmaf(poly, t, 0.0994652063f);
+    poly = fmaf(poly, t, 0.120826296f);
+    poly = fmaf(poly, t, 0.119624548f);
+    *gauss = exp2_approx(-0.5f * kLog2e * (z * z));
+    return poly * t * *gauss;
 }
 
 // 1 / (1 + exp(-w)): the gate of silu (w = z) and of gelu_tanh. Each has its own arithmetic: silu as the other with

@@ -63,3 +63,71 @@ def test_slopes_at_infinity(cuda_device):
         api.hgemm_linear_backward(dC, A, B, act=act, pre=pre, dZ=dZ, dbias=dbias)
         assert (dZ[:, 0::2] == 1.5).all() and (dZ[:, 1::2] == 0).all(), act
         assert (dbias[0::2] == 1.5).all() and (dbias[1::2] == 0).all(), act
+
+
+# ------------------------------------------------------------------------------------------------ the activations' tails
+def smooth64(z, act):
+    """Value and slope in 64 bits without cancellation for negative z, and what FP32 arithmetic may lose of the gate (relative).
+
+    The gate is Phi(z) for gelu and a logistic function else: an exponential of an argument a that is formed by up to six
+    roundings to FP32 (constants included), each 2^-24 |a| absolute, hence relative in the exponential; the hardware's
+    exponential and reciprocal, 2^-22 each; gelu's polynomial (1.2e-7 and at most four FP32 roundings) and three products: 2^-20
+    covers them."""
+    import math
+
+    import torch
+
+    if act == "gelu":
+        gate, a = 0.5 * torch.special.erfc(-z * math.sqrt(0.5)), z * z / 2
+        slope = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    else:
+        w = z if act == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+        dw = torch.ones_like(z) if act == "silu" else 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+        gate, a = torch.sigmoid(w), w.abs()
+        slope = gate * torch.sigmoid(-w) * dw
+    return gate, slope, 2.0 ** -20 + 6 * 2.0 ** -24 * a
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [16, 256])  # the short-A kernels, the grouped kernel
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_activations_in_fp32_relative_to_their_value(cuda_device, dtype, rows, act):
+    """A product with the identity hands every z of a grid over [-6, 6] on exactly; C in FP32 is then the activation alone."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    N = 4096 if rows == 16 else 64
+    A = torch.linspace(-6, 6, rows * 64, device=cuda_device).view(rows, 64).to(torch_type(dtype))
+    B = torch.eye(64, device=cuda_device).to(A.dtype).repeat(N // 64, 1)
+    C = torch.full((rows, N), float("nan"), device=cuda_device)
+    api.hgemm_linear(A, B, C, act=act)
+    z = A.double().repeat(1, N // 64)
+    gate, _, rel = smooth64(z, act)
+    # (1 - tail for positive z: one more rounding; the product with z another)
+    over = (C.double() - z * gate).abs() - (rel + 2.0 ** -22) * (z * gate).abs()
+    at = over.argmax()
+    assert over.max() <= 0, (z.flatten()[at].item(), C.flatten()[at].item(), (z * gate).flatten()[at].item())
+    assert api.last_device_error() == 0
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_slopes_in_fp32_relative_to_their_terms(cuda_device, act):
+    """With one row and a gradient of one, dbias is the slope itself: gate + z gate', each term to its own relative bound."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    N, K = 8192, 8
+    A, B = torch.zeros((1, K), dtype=torch.bfloat16, device=cuda_device), torch.zeros((N, K), dtype=torch.bfloat16, device=cuda_device)
+    pre = torch.linspace(-6, 6, N, device=cuda_device).view(1, N)
+    dbias = torch.empty(N, device=cuda_device)
+    api.hgemm_linear_backward(torch.ones_like(pre), A, B, act=act, pre=pre, dbias=dbias)
+    z = pre[0].double()
+    gate, slope, rel = smooth64(z, act)
+    # (for positive z the logistic form takes 1 - gate, whose error is that of the gate: 2^-20 of 1 and not of 1 - gate)
+    factor = torch.zeros_like(z) if act == "gelu" else z.abs() * gate * (slope / (gate * (1 - gate).clamp(min=1e-30)))
+    bound = (rel + 2.0 ** -22) * (gate + (z * slope).abs()) + torch.where(z > 0, factor * 2.0 ** -20, 0.0)
+    over = (dbias.double() - (gate + z * slope)).abs() - bound
+    at = over.argmax()
+    assert over.max() <= 0, (z[at].item(), dbias[at].item(), (gate + z * slope)[at].item(), bound[at].item())
