@@ -25,7 +25,8 @@ EXPORTED_SYMBOLS = (
     "b200_hgemm_release_workspaces", "b200_hgemm_synchronize", "b200_hgemm_streamk_static_last_error",
     "b200_debug_wait_expiry_static", "b200_hgemm_fused_ex", "b200_hgemm_batched", "b200_hgemm_bkn", "b200_hgemm_host_a_after", "b200_sched_tile_coord_fast", "b200_debug_fast_div", "b200_debug_cluster_capacity",
     "b200_hgemm_linear", "b200_hgemm_linear_workspace_bytes", "b200_hgemm_linear_backward", "b200_hgemm_grouped",
-    "b200_hgemm_grouped_backward", "b200_hgemm_backward_workspace_bytes",
+    "b200_hgemm_grouped_backward", "b200_hgemm_backward_workspace_bytes", "b200_debug_skinny_start",
+    "b200_debug_early_skinny_launches",
 )
 
 OK = 0
@@ -171,6 +172,10 @@ def load() -> ctypes.CDLL:
     lib.b200_sched_tile_coord_fast.restype = None
     lib.b200_debug_cluster_capacity.argtypes = [c_int]
     lib.b200_debug_cluster_capacity.restype = None
+    lib.b200_debug_skinny_start.argtypes = [c_int, c_int, POINTER(c_uint32)]
+    lib.b200_debug_skinny_start.restype = c_int
+    lib.b200_debug_early_skinny_launches.argtypes = []
+    lib.b200_debug_early_skinny_launches.restype = c_uint64
     lib.b200_debug_fast_div.argtypes = [c_uint32, c_uint32]
     lib.b200_debug_fast_div.restype = c_uint32
     lib.b200_sched_segments.argtypes = [c_uint32, c_uint32, c_uint32, c_uint32, POINTER(c_uint32), c_uint32]

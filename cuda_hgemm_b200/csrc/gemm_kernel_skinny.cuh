@@ -57,7 +57,7 @@ struct alignas(64) SkinnyParams {
     uint32_t n_pad;          // row pitch of the partial results, in floats
     uint32_t tma_store;      // 1: whole results leave through tm_c
     uint32_t prefetch_kb;    // k-blocks of B asked into L2 before waiting for the previous kernel
-    uint32_t after_all;      // host only: launch without overlap with the kernel before
+    uint32_t after_all;      // 1: started when the kernel before has ended; the next one is not let in before this has
     EpilogueArgs epi;        // kernels instantiated with EPI: alpha / beta / bias / c_in and the element type of C
 #ifdef B200_TIMELINE
     unsigned long long *timeline;  // profiling builds only: 32 words per CTA (see GemmParams::timeline)
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) hgemm_skinny_kernel(const __grid_
     }
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = (CG == 1 && warp == 0) ? 0u : *tmem_slot;
-    pdl_launch_dependents();
+    if (!EPI || !p.after_all) pdl_launch_dependents();
     if (threadIdx.x == 0) B200_STAMP(1);
     uint32_t ready = 1;  // epilogue warps: the accumulator is complete
 

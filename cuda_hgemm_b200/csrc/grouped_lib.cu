@@ -27,9 +27,10 @@ static bool misaligned(std::initializer_list<const void *> ptrs) {
     return (bits & 15u) != 0;
 }
 
-// All kernels here are launched plainly, each when the one before it in the stream has ended. Started early
-// (programmatic dependent launch, 1 to 2 us less between two of them) and waiting beside one another, the small
-// CTAs of the pass over dC and the whole-SM CTAs and pairs of the products have been seen to stand still for good.
+// All kernels here are launched plainly, each when the one before it in the stream has ended, and so are the short-A
+// kernels of a linear layer (skinny_start in hgemm_lib.cu). Started early (programmatic dependent launch, 1 to 2 us less between
+// two of them) and waiting beside one another, the small CTAs of the pass over dC and the whole-SM CTAs and pairs of
+// the products have been seen to stand still for good; the cause is not known.
 static void pair_attribute(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr) {
     attr->id = cudaLaunchAttributeClusterDimension;
     attr->val.clusterDim.x = 2;

@@ -951,20 +951,41 @@ static size_t skinny_workspace_bytes(const b200_hgemm_plan &pl, const DeviceStat
     return static_cast<size_t>(slices) * pl.bn * n_pad * sizeof(float);
 }
 
+// How a short-A kernel stands in its stream.
+struct SkinnyStart {
+    bool early;            // its set-up may overlap the end of the kernel before it, and the next kernel's its own end
+    uint32_t prefetch_kb;  // k-blocks of B asked into L2 meanwhile
+};
+
 // k-blocks of B a short-A CTA asks into L2 before it waits for the previous kernel (B200_HGEMM_SKINNY_PREFETCH
 // overrides it for measurements; 0 switches the prefetch off). Without programmatic dependent launch there
 // is no previous kernel to overlap with. Measured inside CUDA graphs, B from HBM: tiles of 16 and 32 rows of A
 // are fastest with 6 ... 8 k-blocks (M = 16: -4 % against none; 32 and more lose), tiles of 64 and 128 rows
 // with 4 (against 8: 22.5 / 22.8 us at M = 64 and 24.7 / 25.2 at M = 128 for N = 14336, 23.0 / 23.8 and
 // 26.0 / 26.6 for N = 4096, K = 14336).
-static uint32_t skinny_prefetch_kb(int rows_per_tile) {
+//
+// The kernels of a linear layer, of one k-range or several and on single CTAs or pairs, start when the kernel before them
+// has ended and let none start beside them: they stand between the pair kernels and the small CTAs of a layer's gradients, and chains of such
+// kernels that started early have been seen to stand still for good (grouped_lib.cu).
+static SkinnyStart skinny_start(bool linear, int rows_per_tile) {
     static const int forced = []() -> int {
         const char *v = getenv("B200_HGEMM_SKINNY_PREFETCH");
         return v ? atoi(v) : -1;
     }();
-    if (!pdl_enabled()) return 0u;
-    if (forced >= 0) return static_cast<uint32_t>(forced);
-    return rows_per_tile >= 64 ? 4u : 8u;
+    if (linear || !pdl_enabled()) return {false, 0u};
+    if (forced >= 0) return {true, static_cast<uint32_t>(forced)};
+    return {true, rows_per_tile >= 64 ? 4u : 8u};
+}
+
+static std::atomic<uint64_t> g_early_skinny_launches{0};  // b200_debug_early_skinny_launches()
+
+// Gives a short-A launch the attribute of an early start; the number of attributes added.
+static int add_early_start(cudaLaunchAttribute *attr, bool early) {
+    if (!early) return 0;
+    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr->val.programmaticStreamSerializationAllowed = 1;
+    g_early_skinny_launches.fetch_add(1, std::memory_order_relaxed);
+    return 1;
 }
 
 static std::atomic<int> g_debug_cluster_capacity{0};  // b200_debug_cluster_capacity(): > 0 overrides what the device reports
@@ -1008,12 +1029,7 @@ static int launch_skinny_kernel(DeviceState &st, int attr_slot, const SkinnyPara
     cfg.dynamicSmemBytes = T::kSmemBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attrs[2];
-    int n_attrs = 0;
-    if (pdl_enabled() && !(CK && p.after_all)) {
-        attrs[n_attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[n_attrs].val.programmaticStreamSerializationAllowed = 1;
-        ++n_attrs;
-    }
+    int n_attrs = add_early_start(attrs, !p.after_all);
     if (CG == 2 || CK) {  // the grid is a whole number of pairs (n_tiles is even), or of clusters of one tile's k-ranges
         attrs[n_attrs].id = cudaLaunchAttributeClusterDimension;
         attrs[n_attrs].val.clusterDim.x = CK ? p.slices * CG : 2;
@@ -1064,10 +1080,9 @@ static int run_skinny(DeviceState &st, const void *A, const void *B, void *C, si
         const int erc = epilogue_args(*epi, &p.epi);
         if (erc != B200_HGEMM_OK) return erc;
     }
-    // Clusters of k-ranges in a linear layer start when the kernel before them has ended, not while it drains: they may
-    // follow the pair kernels of the gradients, and a kernel of small clusters launched programmatically behind one of
-    // those, another pair kernel behind it, has been seen never to end.
-    p.after_all = fused && epi->linear ? 1u : 0u;
+    const SkinnyStart start = skinny_start(fused && epi->linear, pl.bn);
+    p.after_all = start.early ? 0u : 1u;
+    p.prefetch_kb = start.prefetch_kb;
     p.c = static_cast<__half *>(C);
     p.error_word = error_word;
     p.m = static_cast<uint32_t>(M);
@@ -1081,7 +1096,6 @@ static int run_skinny(DeviceState &st, const void *A, const void *B, void *C, si
     p.slices = skinny_slices(pl, st, N, K);
     p.kb_per_slice = ceil_div_u32(p.k_blocks, p.slices);
     p.n_pad = static_cast<uint32_t>((N + 31) / 32 * 32);
-    p.prefetch_kb = skinny_prefetch_kb(pl.bn);
 #ifdef B200_TIMELINE
     p.timeline = g_timeline;
 #endif
@@ -1140,10 +1154,8 @@ static int run_skinny(DeviceState &st, const void *A, const void *B, void *C, si
     cfg.blockDim = dim3(kSkinnyReduceThreads, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    cfg.numAttrs = add_early_start(&attr, start.early);
     if (!cuda_ok(cudaLaunchKernelEx(&cfg, skinny_reduce_kernel, static_cast<const float *>(p.partials), p.c, p.m, p.n, p.n_pad,
                                     static_cast<uint32_t>(pl.bn), p.slices, fused ? 1u : 0u, p.epi),
                  "cudaLaunchKernelEx")) {
@@ -2440,6 +2452,16 @@ void b200_sched_tile_coord_fast(uint32_t tile, uint32_t m_blocks, uint32_t n_blo
 
 void b200_debug_cluster_capacity(int clusters) {
     g_debug_cluster_capacity.store(clusters > 0 ? clusters : 0, std::memory_order_relaxed);
+}
+
+int b200_debug_skinny_start(int linear, int rows_per_tile, uint32_t *prefetch_kb) {
+    const SkinnyStart start = skinny_start(linear != 0, rows_per_tile);
+    if (prefetch_kb) *prefetch_kb = start.prefetch_kb;
+    return start.early ? 1 : 0;
+}
+
+uint64_t b200_debug_early_skinny_launches(void) {
+    return g_early_skinny_launches.load(std::memory_order_relaxed);
 }
 
 uint32_t b200_debug_fast_div(uint32_t n, uint32_t d) {

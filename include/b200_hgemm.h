@@ -377,6 +377,10 @@ int b200_debug_wait_expiry_static(uint32_t limit_ms, b200_stream_t stream);
  * only that many thread-block clusters at once, whatever their size, so its own choice of summing k-ranges inside
  * clusters gives way to the workspace form when there are more clusters than that; 0 restores what the device says. */
 void b200_debug_cluster_capacity(int clusters);
+/* Whether a short-A kernel (tiles of `rows_per_tile` rows) may start while the kernel before it in the stream drains, and
+ * how many k-blocks of B it then asks into L2; never as part of a linear layer. And how many such launches there were. */
+int b200_debug_skinny_start(int linear, int rows_per_tile, uint32_t *prefetch_kb);
+uint64_t b200_debug_early_skinny_launches(void);
 /* tcgen05 descriptor encoders (instruction descriptor; shared-memory matrix descriptor). */
 uint32_t b200_debug_idesc(uint32_t m, uint32_t n);
 uint64_t b200_debug_smem_desc(uint32_t smem_addr);

@@ -131,3 +131,32 @@ def test_slopes_in_fp32_relative_to_their_terms(cuda_device, act):
     over = (dbias.double() - (gate + z * slope)).abs() - bound
     at = over.argmax()
     assert over.max() <= 0, (z[at].item(), dbias[at].item(), (gate + z * slope)[at].item(), bound[at].item())
+
+
+# ------------------------------------------------------------------------------------------------ launches
+def test_no_launch_of_a_linear_layer_starts_early(cuda_device, native_lib):
+    """Short-A kernels of one k-range, of ranges summed inside clusters, of ranges summed through the workspace, and on pairs: none
+    starts while the kernel before it drains. The same shapes through the older entry point do."""
+    import ctypes
+
+    import torch
+
+    from cuda_hgemm_b200 import _native, api
+
+    forms = set()
+    for M, N, K in ((1, 1024, 1024), (16, 14336, 4096), (16, 4096, 14336), (64, 1024, 8192), (100, 512, 4096), (128, 4096, 14336),
+                    (128, 4096, 8192), (64, 14336, 4096)):
+        A, B = torch.zeros((M, K), dtype=torch.float16, device=cuda_device), torch.zeros((N, K), dtype=torch.float16, device=cuda_device)
+        C = torch.full((M, N), SENTINEL, dtype=torch.float16, device=cuda_device)
+        args = _native.LinearArgs(in_type=_native.C_F16, c_type=_native.C_F16, act=_native.ACT_SILU)
+        before = native_lib.b200_debug_early_skinny_launches()
+        api.hgemm_linear(A, B, C, act="silu")
+        assert native_lib.b200_debug_early_skinny_launches() == before, (M, N, K)
+        assert (C == 0).all()
+        torch.cuda.synchronize()
+        api.b200Hgemm(A, B, C)
+        torch.cuda.synchronize()
+        early = native_lib.b200_debug_early_skinny_launches() - before
+        forms.add((early, native_lib.b200_hgemm_linear_workspace_bytes(M, N, K, ctypes.byref(args)) > 0))
+    assert (1, False) in forms and (2, True) in forms  # one kernel, and a kernel with its sum behind it
+    assert api.last_device_error() == 0

@@ -158,3 +158,10 @@ def test_fast_tile_raster_agrees_with_the_plain_one(native_lib):
             native_lib.b200_sched_tile_coord(t, mb, nb, min(g, mb), ctypes.byref(m), ctypes.byref(n))
             native_lib.b200_sched_tile_coord_fast(t, mb, nb, min(g, mb), ctypes.byref(m2), ctypes.byref(n2))
             assert (m.value, n.value) == (m2.value, n2.value), (mb, nb, g, t)
+
+
+def test_short_a_kernels_start_early_except_in_linear_layers(native_lib):
+    prefetch = ctypes.c_uint32(77)
+    for rows, blocks in ((16, 8), (32, 8), (64, 4), (128, 4)):
+        assert native_lib.b200_debug_skinny_start(0, rows, ctypes.byref(prefetch)) == 1 and prefetch.value == blocks
+        assert native_lib.b200_debug_skinny_start(1, rows, ctypes.byref(prefetch)) == 0 and prefetch.value == 0
