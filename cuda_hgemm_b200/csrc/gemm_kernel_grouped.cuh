@@ -17,11 +17,14 @@
 // 904 us against 797). The weight gradient sums over the group's rows: both operands are then row-contiguous in the
 // other index and read by the MMA as MN-major; the accumulator is not transposed.
 //
-// FP32 results of long sums (LONG): the tensor cores cut off what an accumulator cannot hold instead of rounding
-// it, a relative 1.7e-6 after 128 MMAs (a sum of 2048) and growing with the length. That is nothing next to
-// a 16-bit result's rounding, but 30 times FP32's own. Those sums are cut into pieces of kLongBlocks k-blocks that
-// alternate between the two accumulators, and the epilogue warps add the pieces in registers, rounding to nearest
-// (pieces of 1024: 0.8 to 1.0e-6 whatever the length; of 512, as here, half of that).
+// Long sums (LONG): the tensor cores cut off what an accumulator cannot hold instead of rounding it, so that a result
+// shrinks with the number of MMAs: by 1.3e-5 of itself per 2048 positive terms, 2e-6 per 2048 of mixed signs (measured from 2048
+// to 131072, in proportion to the length). That is 200 and 30 times FP32's own rounding after 2048; an FP16 result's half step, 4.9e-4, is
+// reached after 77 000 positive terms, BF16's after 610 000. Sums too long for the result's type (longest_sum in lib_state.h)
+// are cut into pieces that alternate between the two accumulators, and the epilogue warps add the pieces in registers, rounding
+// to nearest. FP32: pieces of 512, an error of 0.5e-6 for mixed signs whatever the length (of 1024: 0.8 to 1.0e-6). 16-bit
+// results: pieces of 4096 and 32768 (512 x 1024 x 32768 in FP16: 94 us in one sum, 96 in such
+// pieces, 118 in pieces of 512).
 //
 // Group sizes are known on the device only (a router wrote them): every CTA reads the offsets, cuts the groups
 // into tiles and walks its share of them. Offsets that are out of order or past T are held within [0, T].
@@ -54,7 +57,6 @@ enum GroupedForm : int {
 
 constexpr int kGroupedEpiWarps = 8;
 constexpr int kGroupedThreads = 64 + 32 * kGroupedEpiWarps;
-constexpr uint32_t kLongBlocks = kLongSum / 64;  // k-blocks summed by the tensor cores before the piece is added up in FP32
 constexpr uint32_t kGroupedMaxGroups = 1024;
 constexpr uint32_t kGroupedBand = 8;  // blocks of rows a band of tiles is high
 
@@ -83,6 +85,7 @@ struct alignas(64) GroupedParams {
     uint32_t act;
     uint32_t accumulate;   // weight, FP32: add to the output
     uint32_t slice_rows;   // weight, dense: "group" g is rows [g, g + 1) * slice_rows of one long sum (0: groups as `offsets` says)
+    uint32_t piece_shift;  // LONG: a piece is 1 << piece_shift k-blocks
     uint32_t p_wide, q_wide;  // weight: the operand's map takes two boxes with one copy (load_columns)
 };
 
@@ -92,8 +95,7 @@ struct GroupedTraits {
     static_assert(CG == 1 || CG == 2, "single CTAs or CTA pairs");
     static_assert(QT == 32 || QT == 64 || QT == 128 || QT == 256, "columns of an accumulator");
     static_assert(!kWeight || (QT / CG == 128 && KPS == 1), "weight form: two 64-column boxes of Q per CTA");
-    static_assert(!LONG || FORM != kFormInput, "the input's gradient is 16-bit");
-    static_assert(kLongBlocks % KPS == 0, "whole stages per piece of a long sum");
+    static_assert((kLongSumF32 / 64u) % KPS == 0, "whole stages per piece of a long sum");
     static constexpr uint32_t kChunk = QT >= 64 ? 32 : 16;  // accumulator columns an epilogue warp takes at a time
     static constexpr uint32_t kStep = 16u * CG;  // an MMA's columns come in these steps
     static constexpr uint32_t kPBytes = 128u * 128u;
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                     tcgen05_fence_after_sync();
                     uint32_t begun = 0;  // 1: the accumulator holds a part of this piece
                     for (uint32_t kb = 0; ok && kb < whole; ++kb) {
-                        if (LONG && kb != 0 && kb % (kLongBlocks / KPS) == 0) {
+                        if (LONG && kb != 0 && ((kb * KPS) & ((1u << p.piece_shift) - 1u)) == 0) {
                             // the next piece, in the other accumulator
                             if (CG == 1) umma_commit(tfull_bar + 8u * (it & 1u)); else umma_commit_pair(tfull_bar + 8u * (it & 1u), 0x3);
                             ++it;
@@ -718,11 +720,15 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                 }
             }
             uint32_t run[LONG ? kChunks * W : 1];
+            // LONG: first column of group i of 16 running sums. The two warps of a quadrant alternate every `span` columns:
+            // a chunk, or, in the weight form, what 128 bytes of a row of the result take.
+            const uint32_t span = WEIGHT && p.out_type != 2u ? 64u : W;
+            auto run_column = [&](uint32_t i) -> uint32_t { return (2u * (i * 16u / span) + half) * span + i * 16u % span; };
             if constexpr (LONG) {
                 const uint32_t k_blocks = WEIGHT ? (tile.valid + kStepK - 1u) / kStepK : p.k_blocks * KPS;
                 // (a tail joins the last piece, so pieces are counted over the whole blocks)
                 const uint32_t whole = WEIGHT ? tile.valid / kStepK : k_blocks;
-                const uint32_t pieces = max((whole + kLongBlocks - 1u) / kLongBlocks, k_blocks != 0 ? 1u : 0u);
+                const uint32_t pieces = max((whole + (1u << p.piece_shift) - 1u) >> p.piece_shift, k_blocks != 0 ? 1u : 0u);
 #pragma unroll
                 for (uint32_t j = 0; j < kChunks * W; ++j) run[j] = 0u;
                 for (uint32_t piece = 0; alive && piece < pieces; ++piece) {
@@ -730,7 +736,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                     if (!alive) break;
 #pragma unroll
                     for (uint32_t c = 0; c < kChunks * W / 16u; ++c) {
-                        const uint32_t at = (2u * (c * 16u / W) + half) * W + c * 16u % W;
+                        const uint32_t at = run_column(c);
                         if (at < cols) {
                             uint32_t r[16];
                             tmem_ld_32x32b_x16(lanes + (it & 1u) * QT + at, r);
@@ -753,7 +759,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                     if constexpr (LONG) {
 #pragma unroll
                         for (uint32_t i = 0; i < kChunks * W / 16u; ++i) {  // (16 at a time: the running sums leave few registers)
-                            const uint32_t at = (2u * (i * 16u / W) + half) * W + i * 16u % W;
+                            const uint32_t at = run_column(i);
                             if (at < cols) finish_rows<FORM, 16>(p, run + i * 16u, bias, tile.q0 + at, cols - at, col, col_end, lane);
                         }
                     } else {
@@ -790,14 +796,39 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                         *reinterpret_cast<uint4 *>(row_ptr + ((j ^ (lane & 7u)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
                     }
                 };
-                if constexpr (LONG) {
+                // 32 values of this lane's row, as part 0 or 1 of its 128 bytes
+                auto put_16 = [&](const uint32_t *r, uint32_t part) {
 #pragma unroll
-                    for (uint32_t i = 0; i < kChunks; ++i) {
-                        const uint32_t at = (2u * i + half) * W;
-                        if (at < cols) {
-                            staging_free();
-                            put_f32(run + i * W);
-                            send(at);
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        uint4 v;
+                        v.x = pack2_typed(r[8 * j + 0], r[8 * j + 1], p.out_type);
+                        v.y = pack2_typed(r[8 * j + 2], r[8 * j + 3], p.out_type);
+                        v.z = pack2_typed(r[8 * j + 4], r[8 * j + 5], p.out_type);
+                        v.w = pack2_typed(r[8 * j + 6], r[8 * j + 7], p.out_type);
+                        *reinterpret_cast<uint4 *>(row_ptr + (((part * 4u + j) ^ (lane & 7u)) << 4)) = v;
+                    }
+                };
+                if constexpr (LONG) {
+                    if (p.out_type == 2u) {
+#pragma unroll
+                        for (uint32_t i = 0; i < kChunks; ++i) {
+                            const uint32_t at = (2u * i + half) * 32u;
+                            if (at < cols) {
+                                staging_free();
+                                put_f32(run + i * 32u);
+                                send(at);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < kChunks / 2u; ++i) {
+                            const uint32_t at = (2u * i + half) * 64u;
+                            if (at < cols) {
+                                staging_free();
+                                put_16(run + i * 64u, 0);
+                                put_16(run + i * 64u + 32u, 1);
+                                send(at);
+                            }
                         }
                     }
                 } else {
@@ -819,15 +850,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
                             if (f32) {
                                 put_f32(r);
                             } else {
-#pragma unroll
-                                for (uint32_t j = 0; j < 4; ++j) {
-                                    uint4 v;
-                                    v.x = pack2_typed(r[8 * j + 0], r[8 * j + 1], p.out_type);
-                                    v.y = pack2_typed(r[8 * j + 2], r[8 * j + 3], p.out_type);
-                                    v.z = pack2_typed(r[8 * j + 4], r[8 * j + 5], p.out_type);
-                                    v.w = pack2_typed(r[8 * j + 6], r[8 * j + 7], p.out_type);
-                                    *reinterpret_cast<uint4 *>(row_ptr + (((part * 4u + j) ^ (lane & 7u)) << 4)) = v;
-                                }
+                                put_16(r, part);
                             }
                         }
                         send(at);

@@ -40,6 +40,14 @@ static void pair_attribute(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr) {
     cfg->numAttrs = 1;
 }
 
+// Whether a result's sum of `length` products is added up from pieces, and, if so, how long those are.
+static bool sum_in_pieces(GroupedParams &p, size_t length) {
+    const int32_t type = static_cast<int32_t>(p.out_type);
+    const uint32_t blocks = sum_piece(type) / 64u;  // a power of two
+    while ((1u << p.piece_shift) < blocks) ++p.piece_shift;
+    return length > longest_sum(type);
+}
+
 // `most_tiles`: an upper bound of the tiles there can be; the grid is persistent and never larger than what
 // is resident at once.
 template <int FORM, int CG, int QT, int STAGES, int KPS, bool LONG = false>
@@ -163,14 +171,12 @@ static int run_rows(DeviceState &st, const void *X, const void *W, size_t rows, 
         if ((rc = get_tensor_map(st, X, rows, k_dim, 16u * (i + 1u), 64, &p.tm_q[i])) != B200_HGEMM_OK) return rc;
     }
     const int slot = kSlots + static_cast<int>(plan.kernel);
-    if constexpr (FORM == kFormForward) {
-        if (p.out_type == B200_C_F32 && k_dim > kLongSum) {
-            switch (plan.kernel) {
-                case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, stream);
-                case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, stream);
-                case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, stream);
-                default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, stream);
-            }
+    if (sum_in_pieces(p, k_dim)) {
+        switch (plan.kernel) {
+            case kRowsPair256: return launch_grouped<FORM, 2, 256, 6, 1, true>(st, slot + 4, p, tiles, stream);
+            case kRowsPair128: return launch_grouped<FORM, 2, 128, 4, 2, true>(st, slot + 4, p, tiles, stream);
+            case kRowsSingle128: return launch_grouped<FORM, 1, 128, 3, 2, true>(st, slot + 4, p, tiles, stream);
+            default: return launch_grouped<FORM, 1, 32, 5, 2, true>(st, slot + 4, p, tiles, stream);
         }
     }
     switch (plan.kernel) {
@@ -264,10 +270,11 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
     if ((rc = columns_map(st, dZ, M, N, &p.tm_p, &p.p_wide)) != B200_HGEMM_OK) return rc;
     if ((rc = columns_map(st, A, M, K, &p.tm_q[0], &p.q_wide)) != B200_HGEMM_OK) return rc;
     const bool f32 = p.out_type == B200_C_F32;
+    const bool in_pieces = sum_in_pieces(p, longest);
     if ((rc = get_tensor_map(st, p.out, N, K, 32, f32 ? 32 : 64, &p.tm_out, true, G, N * K, f32 ? 4 : 2)) != B200_HGEMM_OK) return rc;
     if (slices > 1) {
-        rc = longest > kLongSum ? launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, stream)
-                                : launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, stream);
+        rc = in_pieces ? launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 113, p, tiles, stream)
+                       : launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 115, p, tiles, stream);
         if (rc != B200_HGEMM_OK) return rc;
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
@@ -283,12 +290,12 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
         g_launches.fetch_add(1, std::memory_order_relaxed);
         return B200_HGEMM_OK;
     }
-    if (f32 && M > kLongSum) {
-        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 108, p, tiles, stream);
-        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 109, p, tiles, stream);
+    if (in_pieces) {
+        if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1, true>(st, 112, p, tiles, stream);
+        return launch_grouped<kFormWeight, 1, 128, 5, 1, true>(st, 113, p, tiles, stream);
     }
-    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 110, p, tiles, stream);
-    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 111, p, tiles, stream);
+    if (cg == 2) return launch_grouped<kFormWeight, 2, 256, 6, 1>(st, 114, p, tiles, stream);
+    return launch_grouped<kFormWeight, 1, 128, 5, 1>(st, 115, p, tiles, stream);
 }
 
 // ---- the pass over dC -----------------------------------------------------------------------

@@ -1855,8 +1855,8 @@ int b200_hgemm_fused_ex(const void *A, const void *B, void *C, size_t M, size_t 
 // activation and with Z beside C. In BF16 with silu, short-A against grouped: 33 x 14336 x 4096 24.8 and 26.3 us, 64
 // rows 23.8 and 25.3, 128 rows 36.2 and 28.7; 64 x 4096 x 14336 26.4 and 35.3; 100 x 2048 x 1024 13.7 and 7.0, 64 x 1024 x 1024
 // 10.3 and 6.7; and 8192 x 14336 x 4096 with gelu and Z 1453 us on the whole-tile kernels with their fused epilogue
-// (one row per lane, values one after the other), 697 on the grouped one. FP32 results of long sums go there too: see
-// gemm_kernel_grouped.cuh.
+// (one row per lane, values one after the other), 697 on the grouped one. Results of sums that are added up in pieces go there
+// too: see gemm_kernel_grouped.cuh.
 // k-ranges summed inside clusters are asked for by name: left to the library they could fall back to a workspace of
 // its own, and this entry point uses the caller's only.
 static bool linear_plan(const DeviceState &st, size_t M, size_t N, size_t K, const b200_linear_args &args, b200_hgemm_plan *pl) {
@@ -1864,7 +1864,7 @@ static bool linear_plan(const DeviceState &st, size_t M, size_t N, size_t K, con
     if (pl->variant != B200_VARIANT_SKINNY && pl->variant != B200_VARIANT_SKINNY_PAIR) return false;
     const uint32_t slices = skinny_slices(*pl, st, N, K);
     if (slices == 1 ? M > 64 : M > 16 && K < 4096) return false;
-    if (args.c_type == B200_C_F32 && K > kLongSum * slices) return false;
+    if (ceil_div_u32(K, slices) > longest_sum(args.c_type)) return false;
     if (pl->grid == 0 && skinny_sums_on_chip(*pl, slices) == 1) pl->grid = 1;
     return true;
 }

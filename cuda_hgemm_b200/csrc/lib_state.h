@@ -84,8 +84,16 @@ int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t col
                    uint64_t pitch = 0, uint32_t box_batch = 1);
 bool pdl_enabled();
 
-// Longest sum an FP32 result may take from one accumulator of the tensor cores (gemm_kernel_grouped.cuh says why).
-constexpr uint32_t kLongSum = 512;
+// Longest sum a result may take from one accumulator of the tensor cores, and the pieces that longer ones are added up
+// from (gemm_kernel_grouped.cuh says why). FP32: 512 and 512. A 16-bit result loses a fifth of the half step that its
+// rounding costs anyway at the longest single sum, and a twentieth in pieces.
+constexpr uint32_t kLongSumF32 = 512, kLongSumF16 = 16384, kLongSumBf16 = 131072;
+inline uint32_t longest_sum(int32_t out_type) {
+    return out_type == B200_C_F32 ? kLongSumF32 : out_type == B200_C_F16 ? kLongSumF16 : kLongSumBf16;
+}
+inline uint32_t sum_piece(int32_t out_type) {
+    return out_type == B200_C_F32 ? kLongSumF32 : longest_sum(out_type) / 4;
+}
 // A linear layer on the grouped kernel, all rows one group (arguments checked by the caller).
 int run_linear_rows(DeviceState &st, const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args &args,
                     cudaStream_t stream);

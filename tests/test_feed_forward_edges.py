@@ -160,3 +160,61 @@ def test_no_launch_of_a_linear_layer_starts_early(cuda_device, native_lib):
         forms.add((early, native_lib.b200_hgemm_linear_workspace_bytes(M, N, K, ctypes.byref(args)) > 0))
     assert (1, False) in forms and (2, True) in forms  # one kernel, and a kernel with its sum behind it
     assert api.last_device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ long sums
+def graded(shape, dtype, device, seed, scale=1.0):
+    """Positive values whose columns (dimension 1) differ in size, so that the results fall anywhere between two steps."""
+    import torch
+
+    gen = torch.Generator(device=device).manual_seed(seed)
+    x = torch.rand(shape, generator=gen, device=device).mul_(0.5).add_(0.5)
+    x *= (torch.rand((1, shape[1]), generator=gen, device=device) * 0.5 + 0.5) * scale
+    return x.to(torch_type(dtype))
+
+
+def mean_signed_error(got, ref):
+    return ((got.double() - ref) / ref).mean().item()
+
+
+LONG = 262144
+
+
+@pytest.mark.parametrize("form", ["forward", "input gradient", "weight gradient", "weight gradient on pairs"])
+@pytest.mark.parametrize("dtype,length", [(F16, LONG), (BF16, 2 * LONG)])
+def test_16_bit_results_of_very_long_sums_do_not_shrink(cuda_device, dtype, length, form):
+    """The tensor cores cut an accumulator off at every MMA (16 terms), which makes a sum of positive terms smaller: by 1e-7 a
+    step, 1.7e-3 after 16384 of them. Longer sums are cut into pieces of 4096 terms (FP16) or 32768
+    (BF16), which lose at most 2^-23 a step. What else can move the mean of `count` results is their one
+    rounding: u / sqrt(3 count) is its standard deviation, four of them are allowed."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    if form == "forward":
+        A, B = graded((136, length), dtype, cuda_device, 1), graded((128, length), dtype, cuda_device, 2, 2.0 ** -6)
+        A, B = A * graded((136, 1), dtype, cuda_device, 3), B * graded((128, 1), dtype, cuda_device, 4)
+        got = torch.empty((136, 128), dtype=A.dtype, device=cuda_device)
+        api.hgemm_linear(A, B, got)
+        ref = A.double() @ B.double().T
+    elif form == "input gradient":
+        dC, B = graded((136, length), dtype, cuda_device, 1), graded((length, 128), dtype, cuda_device, 2, 2.0 ** -6)
+        dC = dC * graded((136, 1), dtype, cuda_device, 3)
+        A, got = torch.empty((136, 128), dtype=dC.dtype, device=cuda_device), torch.empty((136, 128), dtype=dC.dtype, device=cuda_device)
+        api.hgemm_linear_backward(dC, A, B, dA=got)
+        ref = dC.double() @ B.double()
+    else:
+        # one group of rows, whose sum is not cut into slices; enough columns for CTA pairs in the second case
+        N, K = (136, 128) if form == "weight gradient" else (1160, 1096)
+        dC, A = graded((length, N), dtype, cuda_device, 1), graded((length, K), dtype, cuda_device, 2, 2.0 ** -6)
+        B, got = torch.empty((1, N, K), dtype=A.dtype, device=cuda_device), torch.empty((1, N, K), dtype=A.dtype, device=cuda_device)
+        offsets = torch.tensor([0, length], dtype=torch.int32, device=cuda_device)
+        api.hgemm_grouped_backward(dC, A, B, offsets, dB=got)
+        got, ref = got[0], torch.zeros((N, K), dtype=torch.float64, device=cuda_device)
+        for lo in range(0, length, 65536):
+            ref += dC[lo:lo + 65536].double().T @ A[lo:lo + 65536].double()
+    assert torch.isfinite(got).all()
+    u = torch.finfo(got.dtype).eps / 2
+    limit = (256 if dtype == F16 else 2048) * 2.0 ** -23 + 4 * u / (3 * got.numel()) ** 0.5
+    assert abs(mean_signed_error(got, ref)) < limit
+    assert api.last_device_error() == 0
