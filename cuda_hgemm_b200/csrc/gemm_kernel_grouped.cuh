@@ -27,7 +27,8 @@
 // pieces, 118 in pieces of 512).
 //
 // Group sizes are known on the device only (a router wrote them): every CTA reads the offsets, cuts the groups
-// into tiles and walks its share of them. Offsets that are out of order or past T are held within [0, T].
+// into tiles and walks its share of them. Offsets past T are held within [0, T]; where they are out of order, the first two
+// forms let a group begin no earlier than the highest offset before it.
 //
 // A block of rows that reaches past its group's end reads rows of the next group. For P and Q of the first two
 // forms this only adds accumulator columns that are never stored. In the weight gradient those rows are
@@ -162,7 +163,7 @@ __device__ __forceinline__ void rows_tile(const GroupedParams &p, const uint32_t
         if (cum[mid] <= block) lo = mid; else hi = mid;
     }
     const uint32_t first = cum[lo], nq = cum[lo + 1u] - first;
-    const uint32_t start = off[lo], end = max(off[lo + 1u], start), r = end - start;
+    const uint32_t start = off[lo], r = off[lo + 1u] - start;
     uint32_t qb, pb;
     band_coord(t - first * p_blocks, nq, p_blocks, &qb, &pb);
     const uint32_t size = round_up_u32((r + nq - 1u) / nq, 16u * CG);  // even blocks
@@ -391,22 +392,32 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) hgemm_grouped_kernel(const
         }
         __syncthreads();
         if (warp == 0) {
-            // blocks of at most q_max rows before each group: a running sum over 32 groups at a time
-            uint32_t total = 0;
+            // Blocks of at most q_max rows before each group: a running sum over 32 groups at a time. The offsets are put in order by
+            // a running maximum first: the groups then hold no more rows than there are, and the sum fits 32 bits.
+            uint32_t total = 0, high = off[0];
             for (uint32_t g0 = 0; g0 < p.groups; g0 += 32u) {
                 const uint32_t g = g0 + lane;
-                uint32_t blocks = 0;
-                if (g < p.groups) {
-                    const uint32_t start = off[g], end = max(off[g + 1u], start);
-                    blocks = (end - start + p.q_max - 1u) / p.q_max;
+                uint32_t end = g < p.groups ? off[g + 1u] : 0u;
+#pragma unroll
+                for (uint32_t d = 1; d < 32; d <<= 1) {
+                    const uint32_t up = __shfl_up_sync(0xffffffffu, end, d);
+                    if (lane >= d) end = max(end, up);
                 }
+                end = max(end, high);
+                const uint32_t before = __shfl_up_sync(0xffffffffu, end, 1);
+                const uint32_t start = lane == 0 ? high : before;
+                high = __shfl_sync(0xffffffffu, end, 31);
+                const uint32_t blocks = (end - start + p.q_max - 1u) / p.q_max;  // (none past the last group: end is start)
                 uint32_t sum = blocks;
 #pragma unroll
                 for (uint32_t d = 1; d < 32; d <<= 1) {
                     const uint32_t up = __shfl_up_sync(0xffffffffu, sum, d);
                     if (lane >= d) sum += up;
                 }
-                if (g < p.groups) cum[g] = total + sum - blocks;
+                if (g < p.groups) {
+                    cum[g] = total + sum - blocks;
+                    off[g + 1u] = end;
+                }
                 total += __shfl_sync(0xffffffffu, sum, 31);
             }
             if (lane == 0) cum[p.groups] = total;

@@ -4,7 +4,7 @@ sums of hundreds of thousands of terms.
 Each test derives its own bound; u(t) is half a step of type t relative to the value: FP16 2^-11, BF16 2^-8, FP32 2^-24."""
 import pytest
 
-from tests.test_feed_forward import ACTS, BF16, F16, F32, SENTINEL, act64
+from tests.test_feed_forward import ACTS, BF16, F16, F32, SENTINEL, act64, check_forward, make
 
 pytestmark = pytest.mark.gpu
 
@@ -217,4 +217,31 @@ def test_16_bit_results_of_very_long_sums_do_not_shrink(cuda_device, dtype, leng
     u = torch.finfo(got.dtype).eps / 2
     limit = (256 if dtype == F16 else 2048) * 2.0 ** -23 + 4 * u / (3 * got.numel()) ** 0.5
     assert abs(mean_signed_error(got, ref)) < limit
+    assert api.last_device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ offsets
+def test_offsets_out_of_order_over_more_than_a_billion_rows(cuda_device):
+    """Every other offset is 0 and the rest M: taken as they stand, 512 groups of M rows are more blocks of rows than 32 bits count.
+    Put in order, the first group holds every row; nothing behind row M is written."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    M, N, K, G = (1 << 30) + (1 << 27), 8, 8, 1024
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("not enough free memory")
+    A = torch.full((M, K), 0.5, dtype=torch.bfloat16, device=cuda_device)
+    B = make((G, N, K), BF16, cuda_device, 1)
+    room = torch.full((M + 64, N), SENTINEL, dtype=torch.bfloat16, device=cuda_device)
+    offsets = torch.tensor([0, M] * (G // 2) + [0], dtype=torch.int32, device=cuda_device)
+    api.hgemm_grouped(A, B, room[:M], offsets)
+    assert (room[M:] == SENTINEL).all()
+    check_forward(A[:1], B[0], None, None, "none", room[:1], None, "first row")
+    for lo in range(0, M, 1 << 27):
+        assert (room[lo:min(lo + (1 << 27), M)] == room[0]).all(), lo
+    offsets = torch.tensor([0, M - 3] * (G // 2) + [M], dtype=torch.int32, device=cuda_device)
+    api.hgemm_grouped(A, B, room[:M], offsets)
+    check_forward(A[M - 3:], B[G - 1], None, None, "none", room[M - 3:M], None, "last rows")
+    assert (room[:M - 3] == room[0]).view(-1, N)[:: 1 << 12].all() and (room[M:] == SENTINEL).all()
     assert api.last_device_error() == 0
