@@ -4,7 +4,7 @@ sums of hundreds of thousands of terms.
 Each test derives its own bound; u(t) is half a step of type t relative to the value: FP16 2^-11, BF16 2^-8, FP32 2^-24."""
 import pytest
 
-from tests.test_feed_forward import ACTS, BF16, F16, F32, SENTINEL, act64, check_forward, make
+from tests.test_feed_forward import ACTS, BF16, F16, F32, SENTINEL, act64, check_backward, check_forward, make
 
 pytestmark = pytest.mark.gpu
 
@@ -244,4 +244,31 @@ def test_offsets_out_of_order_over_more_than_a_billion_rows(cuda_device):
     api.hgemm_grouped(A, B, room[:M], offsets)
     check_forward(A[M - 3:], B[G - 1], None, None, "none", room[M - 3:M], None, "last rows")
     assert (room[:M - 3] == room[0]).view(-1, N)[:: 1 << 12].all() and (room[M:] == SENTINEL).all()
+    assert api.last_device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ gradients of the weights
+@pytest.mark.parametrize("shape", [(5000, 72, 200), (8191, 264, 136), (3000, 256, 256)], ids=str)
+@pytest.mark.parametrize("dtype,act", [(F16, "none"), (BF16, "none"), (BF16, "gelu")])
+def test_accumulated_over_slices(cuda_device, shape, dtype, act):
+    """Enough rows and few enough tiles for the sum to be cut into slices, which are then added to what dB holds."""
+    import ctypes
+
+    import torch
+
+    from cuda_hgemm_b200 import _native, api
+
+    M, N, K = shape
+    # the slices lie in the workspace: without dZ and dbias nothing else does
+    alone = _native.LinearGrads(in_type=_native.C_F16, c_type=_native.C_F16, db_type=_native.C_F32, dC=256, dB=256)
+    assert _native.load().b200_hgemm_backward_workspace_bytes(M, N, K, 1, ctypes.byref(alone)) >= 2 * 4 * N * K
+    A, B = make((M, K), dtype, cuda_device, 1), make((N, K), dtype, cuda_device, 2)
+    dC, pre = make((M, N), dtype, cuda_device, 3, 0.1), make((M, N), dtype, cuda_device, 4, 2.0)
+    dZ = torch.empty_like(dC) if act != "none" else None
+    was, was_bias = make((N, K), F32, cuda_device, 5, 30.0), make((N,), F32, cuda_device, 6, 30.0)
+    dB, dbias = was.clone(), was_bias.clone()
+    for _ in range(2):  # twice: the second call adds to the first one's result
+        before, before_bias = dB.clone(), dbias.clone()
+        api.hgemm_linear_backward(dC, A, B, act=act, pre=pre if act != "none" else None, dB=dB, dbias=dbias, dZ=dZ, accumulate=True)
+        check_backward(dC, A, B, act, pre, dZ, None, dB, dbias, "slices", dB_was=before, dbias_was=before_bias)
     assert api.last_device_error() == 0
