@@ -358,7 +358,8 @@ def hgemm_linear_backward(dC, A, B, act: str = "none", pre=None, dA=None, dB=Non
     ``dZ = dC * act'(pre)``, ``dA = dZ @ B``, ``dB = dZ.T @ A`` and ``dbias`` the column sums of ``dZ``.
 
     ``dC`` and ``pre`` ``[M, N]`` have the forward pass's C type; ``dA [M, K]`` and ``dZ [M, N]`` the inputs' type, ``dB [N, K]``
-    that type or float32, ``dbias [N]`` float32 (summed before ``dZ`` is rounded for the products). With ``accumulate``
+    that type or float32, ``dbias [N]`` float32 (summed before ``dZ`` is rounded). Both products read ``dZ`` rounded to
+    the inputs' type, so each term of a float32 ``dB`` behind an activation carries that rounding. With ``accumulate``
     the new ``dB`` (float32 then) and ``dbias`` are added to what the tensors hold. The gradient of the residual is
     ``dC``. ``N`` and ``K`` are multiples of 8; ``M`` may be 0. Returns ``(dA, dB, dbias)``."""
     _backward(dC, A, B, None, act, pre, dA, dB, dbias, dZ, accumulate)

@@ -3,6 +3,11 @@
 //   dZ[t][n] = dC[t][n] * act'(Z[t][n])          rounded to the products' 16-bit type
 //   dbias_g[n] = sum over the rows t of group g of the unrounded dZ[t][n]
 //
+// The rounding is what the tensor cores ask for: their operands are 16-bit. It is the only one between dC and the products'
+// FP32 sums; each term of dA's and dB's sums is off by half a step of the inputs' type at most, so an FP32 dB behind an activation
+// (or of an FP32 dC) is as good as 16-bit terms make it, however it is accumulated. Terms of twice the width, as two 16-bit numbers each,
+// would double the time of both products.
+//
 // Bound by HBM: dC and Z are read once, dZ is written once, and the column sums ride along in registers. A
 // block takes 256 columns (a warp reads 512 consecutive bytes of a row) of one slice of a group's rows; its eight
 // warps take every eighth row, eight columns per lane, four rows in flight, which leaves registers for four blocks

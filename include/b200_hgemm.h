@@ -220,7 +220,7 @@ typedef struct b200_linear_grads {
     int32_t in_type;    /* type of A, B, dA and dZ */
     int32_t c_type;     /* type of dC and pre: in_type, or B200_C_F32 */
     int32_t act;        /* B200_ACT_* of the forward pass */
-    int32_t db_type;    /* type of dB: in_type, or B200_C_F32 */
+    int32_t db_type;    /* type of dB: in_type, or B200_C_F32 (FP32 sums of products with dZ rounded to in_type) */
     int32_t accumulate; /* 1: dB and dbias are added to (dB must be B200_C_F32); 0: overwritten */
     const void *dC;     /* M x N */
     const void *pre;    /* M x N: the forward pass's Z; may be NULL when act is B200_ACT_NONE */

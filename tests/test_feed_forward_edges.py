@@ -4,7 +4,8 @@ sums of hundreds of thousands of terms.
 Each test derives its own bound; u(t) is half a step of type t relative to the value: FP16 2^-11, BF16 2^-8, FP32 2^-24."""
 import pytest
 
-from tests.test_feed_forward import ACTS, BF16, F16, F32, SENTINEL, act64, check_backward, check_forward, make
+from tests.test_feed_forward import (ACTS, BF16, F16, F32, SENTINEL, act64, assert_within, check_backward, check_forward, half_step, make, rounded,
+                                     slope64, sum_error)
 
 pytestmark = pytest.mark.gpu
 
@@ -271,4 +272,41 @@ def test_accumulated_over_slices(cuda_device, shape, dtype, act):
         before, before_bias = dB.clone(), dbias.clone()
         api.hgemm_linear_backward(dC, A, B, act=act, pre=pre if act != "none" else None, dB=dB, dbias=dbias, dZ=dZ, accumulate=True)
         check_backward(dC, A, B, act, pre, dZ, None, dB, dbias, "slices", dB_was=before, dbias_was=before_bias)
+    assert api.last_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("sizes", [None, [700, 0, 33, 1290]], ids=["linear", "grouped"])
+def test_products_of_an_unrounded_dz(cuda_device, sizes, act, dtype):
+    """dA and an FP32 dB, accumulated, against dZ in 64 bits. The products read dZ rounded to the inputs' type: each of its values, and
+    with it each term of a sum, is off by u(type) at most, or by half of FP16's smallest step; the slope by 2^-19."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    M, N, K = sum(sizes) if sizes else 1500, 264, 136
+    bounds = [0]
+    for r in sizes or [M]:
+        bounds.append(bounds[-1] + r)
+    G = len(bounds) - 1
+    A, B = make((M, K), dtype, cuda_device, 1), make((G, N, K), dtype, cuda_device, 2, K ** -0.5)
+    dC, pre = make((M, N), dtype, cuda_device, 3), make((M, N), dtype, cuda_device, 4, 2.0)
+    was = make((G, N, K), F32, cuda_device, 5)
+    dA, dB = torch.empty_like(A), was.clone()
+    if sizes:
+        offsets = torch.tensor(bounds, dtype=torch.int32, device=cuda_device)
+        api.hgemm_grouped_backward(dC, A, B, offsets, act=act, pre=pre, dA=dA, dB=dB, accumulate=True)
+    else:
+        api.hgemm_linear_backward(dC, A, B[0], act=act, pre=pre, dA=dA, dB=dB[0], accumulate=True)
+    dz = dC.double() * slope64(pre.double(), act)
+    edz = half_step(dtype) * dz.abs() + 2.0 ** -19 * dC.double().abs() * 1.001 + (2.0 ** -25 if dtype == F16 else 0)
+    for g in range(G):
+        r = slice(bounds[g], bounds[g + 1])
+        a, b, z, ez = A[r].double(), B[g].double(), dz[r], edz[r]
+        err = ez @ b.abs() + sum_error(N, (z.abs() + ez) @ b.abs())
+        assert_within(dA[r], z @ b, rounded(z @ b, err, dtype), f"dA {g}")
+        ref = z.T @ a + was[g].double()
+        err = ez.T @ a.abs() + sum_error(len(a), (z.abs() + ez).T @ a.abs()) + 2.0 ** -23 * (ref.abs() + was[g].double().abs())
+        assert_within(dB[g], ref, rounded(ref, err, torch.float32), f"dB {g}")
     assert api.last_device_error() == 0
