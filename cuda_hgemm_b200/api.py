@@ -56,7 +56,9 @@ def _shape_of(A, B, C, c_dtypes=None):
 def _stream_of(t) -> int:
     import torch
 
-    return torch._C._cuda_getCurrentRawStream(t.get_device())  # (the public call builds a Stream object: 3 us of a call's 17)
+    # torch's own number of the stream where this torch has it; the public call builds a Stream object: 3 us of a call's 17
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(t.get_device()) if raw is not None else int(torch.cuda.current_stream(t.device).cuda_stream)
 
 
 def _call(symbol: str, A, B, C):
