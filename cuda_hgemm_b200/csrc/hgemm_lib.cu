@@ -172,7 +172,7 @@ int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t col
 // is the one setting in which that holds by construction (the reference's model: one device per
 // process, src/main.cu:45,51). Such a process is recognised by
 //   * WORLD_SIZE or LOCAL_WORLD_SIZE > 1 in the environment (one rank of several), or
-//   * a b200_mg_create() call that names two or more devices,
+//   * a b200_mg_create() call that names two or more different devices,
 // and either locks the switch in the off position for the rest of the process's life.
 typedef int (*McLaunchFn)(const void *params, void *stream, int use_pdl);
 
@@ -2286,7 +2286,13 @@ int b200_mg_create(const int *devices, int n, b200_mg **out) {
     if (!devices || !out || n < 1 || n > kMaxDevices) return B200_HGEMM_ERR_INVALID_ARG;
     // A process that sets out to drive several GPUs never runs the kernels with multicast loads;
     // the switch is locked before anything else can fail.
-    if (n >= 2) mc_lock_off();
+    // (A list that names one device several times is refused below and names no second one.)
+    for (int i = 1; i < n; ++i) {
+        if (devices[i] != devices[0]) {
+            mc_lock_off();
+            break;
+        }
+    }
     int count = 0;
     if (!cuda_ok(cudaGetDeviceCount(&count), "cudaGetDeviceCount")) return B200_HGEMM_ERR_CUDA;
     for (int i = 0; i < n; ++i) {

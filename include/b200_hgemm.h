@@ -306,7 +306,7 @@ int b200_hgemm_plan_supported(size_t M, size_t N, size_t K, const b200_hgemm_pla
  * B200_HGEMM_MULTICAST=1 in its environment). They are for processes that own ONE GPU, the
  * reference's model (its only device knob is -gpu_rank, src/main.cu:45,51): in a process that is one
  * rank of several (WORLD_SIZE or LOCAL_WORLD_SIZE > 1) or that has called b200_mg_create() with two or
- * more devices the switch is locked off for good, b200_hgemm_enable_multicast(1) returns
+ * more different devices the switch is locked off for good, b200_hgemm_enable_multicast(1) returns
  * B200_HGEMM_ERR_UNSUPPORTED, b200_hgemm_select() never picks the variant and an explicit plan that
  * names it is refused. Also B200_HGEMM_ERR_UNSUPPORTED when the companion library is absent.
  * b200_hgemm_multicast_state(): 0 = off, 1 = on, 2 = locked off. */

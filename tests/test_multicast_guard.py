@@ -129,3 +129,23 @@ def test_a_handle_on_several_devices_locks_it_off(native_lib):
     assert out["enable"] == _native.ERR_UNSUPPORTED
     assert out["pick"] == [_native.VARIANT_CTA2, 512]
     assert out["explicit"] == _native.ERR_UNSUPPORTED
+
+
+@needs_companion
+def test_a_list_that_names_one_device_twice_does_not_lock_it(native_lib):
+    """Such a list is refused and drives no second GPU, so what runs later in the process may still switch the kernels on; a list
+    that names a second device locks the switch wherever it stands in the list."""
+    out = run_case("""
+        handle = ctypes.c_void_p()
+        for devices in ((0, 0), (0, 0, 0), (-1,), (4096,)):
+            lib.b200_mg_create((ctypes.c_int * len(devices))(*devices), len(devices), ctypes.byref(handle))
+        out["state"] = lib.b200_hgemm_multicast_state()
+        out["enable"] = lib.b200_hgemm_enable_multicast(1)
+        lib.b200_hgemm_enable_multicast(0)
+        lib.b200_mg_create((ctypes.c_int * 3)(0, 0, 1), 3, ctypes.byref(handle))
+        out["after_two"] = lib.b200_hgemm_multicast_state()
+    """)
+    from cuda_hgemm_b200 import _native
+
+    assert out["state"] == _native.MULTICAST_OFF and out["enable"] == _native.OK
+    assert out["after_two"] == _native.MULTICAST_LOCKED_OFF
