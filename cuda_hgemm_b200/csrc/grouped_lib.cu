@@ -109,7 +109,9 @@ struct RowsPlan {
 //   * its MMAs: 1.1 ns per row of the block (1.3 with the whole GPU at work), 128 columns of the result per CTA,
 //   * its operands' way out of L2: 20.5 TB/s for all SMs together;
 // a kernel costs 4 us besides (5.5 where two CTAs have to meet), and 10 ns per row of a block for the last
-// epilogue. Group sizes are not known here: the estimate spreads the rows evenly over the groups.
+// epilogue. Group sizes are not known here: the estimate spreads the rows evenly over the groups, and with 32 rows or fewer
+// on average takes the blocks of 32. One hot expert then reads its weights once per 32 rows: 64 experts of 1024 x 2048, 2048 rows in
+// BF16, take 47 us at 32 rows each and 57 with 1500 rows in one.
 static RowsPlan choose_rows_plan(const DeviceState &st, size_t rows, size_t p_dim, size_t k_dim, size_t groups) {
     const uint64_t live = groups < rows ? groups : rows;  // groups that can hold any rows
     const uint64_t average = (rows + live - 1) / live;
@@ -215,7 +217,7 @@ static int weight_cg(const DeviceState &st, size_t M, size_t N, size_t K, size_t
 }
 
 // Slices a dense layer's long sum over the rows is cut into where its gradient has too few tiles for the GPU: as many as
-// give every SM a tile, of at least 512 rows each. They lie in FP32 in the workspace (20 MB at most) and slice_sum_kernel
+// give every SM a tile, of at least 512 rows each. They lie in FP32 in the workspace (at most 148 tiles of 128 x 128: 9.7 MB) and slice_sum_kernel
 // adds them in order. 8192 rows of 256 x 256: 31 us in one piece, 11 in sixteen; of 1024 x
 // 1024: 33 us, 26 in two.
 static uint32_t weight_slices(size_t M, size_t N, size_t K, size_t G, bool ragged) {
@@ -278,7 +280,7 @@ static int run_weight(DeviceState &st, const void *dZ, const void *A, void *dB, 
         if (rc != B200_HGEMM_OK) return rc;
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
-            const size_t count4 = N * K / 4;
+        const size_t count4 = N * K / 4;
         cfg.gridDim = dim3(ceil_div_u32(count4, 256), 1, 1);
         cfg.blockDim = dim3(256, 1, 1);
         cfg.stream = stream;

@@ -597,7 +597,7 @@ static void select_plan(const DeviceState &st, size_t M, size_t N, size_t K, b20
 // ------------------------------------------------------------------------------------------
 // Programmatic dependent launch is on unless B200_HGEMM_NO_PDL is set in the environment (for
 // A/B measurements; without the launch attribute the kernels' griddepcontrol instructions do nothing).
-bool pdl_enabled() {
+static bool pdl_enabled() {
     static const bool on = (getenv("B200_HGEMM_NO_PDL") == nullptr);
     return on;
 }
@@ -1851,10 +1851,10 @@ int b200_hgemm_fused_ex(const void *A, const void *B, void *C, size_t M, size_t 
 // ---- linear layers --------------------------------------------------------------------------------
 // Whether a linear layer runs on the short-A kernels, with which plan. They take batches of up to 64 rows against
 // enough columns to fill the GPU, batches of up to 128 rows whose long k is cut into ranges (the grouped kernel does not cut
-// it), and any k cut for up to 16 rows (1 x 1024 x 1024: 6.5 us against 8.2). Everything else runs on the grouped kernel as a single group (run_linear_rows), whose epilogue keeps up with an
-// activation and with Z beside C. In BF16 with silu, short-A against grouped: 33 x 14336 x 4096 24.8 and 26.3 us, 64
-// rows 23.8 and 25.3, 128 rows 36.2 and 28.7; 64 x 4096 x 14336 26.4 and 35.3; 100 x 2048 x 1024 13.7 and 7.0, 64 x 1024 x 1024
-// 10.3 and 6.7; and 8192 x 14336 x 4096 with gelu and Z 1453 us on the whole-tile kernels with their fused epilogue
+// it), and any k cut for up to 16 rows (1 x 1024 x 1024: 6.0 us against 7.2). Everything else runs on the grouped kernel as a single group (run_linear_rows), whose epilogue keeps up with an
+// activation and with Z beside C. In BF16 with silu, short-A against grouped in graphs: 33 x 14336 x 4096 24.8 and 27.0 us, 64
+// rows 26.0 and 28.3, 128 rows 36.2 and 28.7; 64 x 4096 x 14336 26.9 and 38.8; 100 x 2048 x 1024 13.7 and 7.0, 64 x 1024 x 1024
+// 10.3 and 6.7; and 8192 x 14336 x 4096 with gelu and Z, in one run, 1453 us on the whole-tile kernels with their fused epilogue
 // (one row per lane, values one after the other), 697 on the grouped one. Results of sums that are added up in pieces go there
 // too: see gemm_kernel_grouped.cuh.
 // k-ranges summed inside clusters are asked for by name: left to the library they could fall back to a workspace of
@@ -1884,11 +1884,12 @@ static int check_linear(const void *A, const void *B, const void *C, size_t M, s
 size_t b200_hgemm_linear_workspace_bytes(size_t M, size_t N, size_t K, const b200_linear_args *args) {
     if (!args || M == 0 || N == 0 || K == 0 || K % 8 != 0) return 0;
     DeviceState *st = nullptr;
-    static DeviceState nominal;
     if (current_state(&st) != B200_HGEMM_OK) {
+        // no usable device: the answer for a B200
         cudaGetLastError();
-        nominal.sm_count = 148;
-        st = &nominal;
+        static DeviceState nominal;
+        static const bool set = (nominal.sm_count = 148) != 0;  // once, whoever comes first
+        if (set) st = &nominal;
     }
     b200_hgemm_plan pl;
     return linear_plan(*st, M, N, K, *args, &pl) ? b200_hgemm_workspace_bytes(M, N, K, &pl) : 0;

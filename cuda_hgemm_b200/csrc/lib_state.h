@@ -82,7 +82,6 @@ int current_state(DeviceState **out);
 int get_tensor_map(DeviceState &st, const void *ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols,
                    CUtensorMap *out, bool swizzle = true, uint64_t batch = 1, uint64_t batch_stride = 0, uint32_t elem_bytes = 2,
                    uint64_t pitch = 0, uint32_t box_batch = 1);
-bool pdl_enabled();
 
 // Longest sum a result may take from one accumulator of the tensor cores, and the pieces that longer ones are added up
 // from (gemm_kernel_grouped.cuh says why). FP32: 512 and 512. A 16-bit result loses a fifth of the half step that its

@@ -12,7 +12,7 @@
 // block takes 256 columns (a warp reads 512 consecutive bytes of a row) of one slice of a group's rows; its eight
 // warps take every eighth row, eight columns per lane, four rows in flight, which leaves registers for four blocks
 // on an SM. What is in flight is kept as it lies in memory: with the values already converted the same kernel
-// reached 2.3 TB/s. 8192 x 14336 in BF16: 142 us with gelu_tanh (705 MB, 4.9 TB/s), 167 us with gelu; eight rows
+// reached 2.3 TB/s. 8192 x 14336 in BF16: 142 us with gelu_tanh (705 MB, 4.9 TB/s), 119 with silu, 208 with gelu; eight rows
 // in flight 173 us, slices of 32 rows 173, of 512 rows 212. The slices' sums are added in order by bias_sum_kernel,
 // so the result does not depend on timing.
 #pragma once

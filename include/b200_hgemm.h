@@ -191,6 +191,8 @@ int b200_hgemm_batched(const void *A, const void *B, void *C, size_t M, size_t N
  * give undefined results but no access outside the operands. M = 0 is allowed everywhere here (there is nothing
  * to write but zero gradients).
  *
+ * An output shares memory with no input and no other output, but where it is said.
+ *
  * Scratch: only what the caller passes (256-byte aligned; the *_workspace_bytes functions say how much, often
  * none), nothing is allocated or kept, so calls on different streams and captured graphs never share any. */
 enum {
@@ -208,7 +210,8 @@ typedef struct b200_linear_args {
     const void *residual; /* M x N, may be C itself, or NULL; the grouped form takes none (B200_HGEMM_ERR_UNSUPPORTED) */
     void *pre;            /* M x N: receives Z, for the backward pass; or NULL */
 } b200_linear_args;
-/* The dispatch is that of b200_hgemm; K % 8 == 0, any N. */
+/* Few rows run on the short-A kernels that b200_hgemm would take, everything else on the grouped kernel as one group;
+ * K % 8 == 0, any N. */
 int b200_hgemm_linear(const void *A, const void *B, void *C, size_t M, size_t N, size_t K, const b200_linear_args *args,
                       void *workspace, size_t workspace_bytes, b200_stream_t stream);
 size_t b200_hgemm_linear_workspace_bytes(size_t M, size_t N, size_t K, const b200_linear_args *args);
