@@ -16,6 +16,20 @@ def torch_type(name):
     return getattr(torch, name)
 
 
+@pytest.fixture
+def most_memory(cuda_device):
+    """GB free once what torch keeps from earlier tests is given back; this test's share is given back too."""
+    import gc
+
+    import torch
+
+    gc.collect()
+    torch.cuda.empty_cache()
+    yield torch.cuda.mem_get_info()[0] >> 30
+    gc.collect()
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------------------------------ infinite Z
 @pytest.mark.parametrize("dtype,out", [(F16, F16), (BF16, BF16), (BF16, F32)])
 @pytest.mark.parametrize("rows", [2, 200])  # the short-A kernels, the grouped kernel
@@ -222,7 +236,7 @@ def test_16_bit_results_of_very_long_sums_do_not_shrink(cuda_device, dtype, leng
 
 
 # ------------------------------------------------------------------------------------------------ offsets
-def test_offsets_out_of_order_over_more_than_a_billion_rows(cuda_device):
+def test_offsets_out_of_order_over_more_than_a_billion_rows(cuda_device, most_memory):
     """Every other offset is 0 and the rest M: taken as they stand, 512 groups of M rows are more blocks of rows than 32 bits count.
     Put in order, the first group holds every row; nothing behind row M is written."""
     import torch
@@ -230,7 +244,7 @@ def test_offsets_out_of_order_over_more_than_a_billion_rows(cuda_device):
     from cuda_hgemm_b200 import api
 
     M, N, K, G = (1 << 30) + (1 << 27), 8, 8, 1024
-    if torch.cuda.mem_get_info()[0] < 60 << 30:
+    if most_memory < 60:
         pytest.skip("not enough free memory")
     A = torch.full((M, K), 0.5, dtype=torch.bfloat16, device=cuda_device)
     B = make((G, N, K), BF16, cuda_device, 1)
@@ -309,4 +323,105 @@ def test_products_of_an_unrounded_dz(cuda_device, sizes, act, dtype):
         ref = z.T @ a + was[g].double()
         err = ez.T @ a.abs() + sum_error(len(a), (z.abs() + ez).T @ a.abs()) + 2.0 ** -23 * (ref.abs() + was[g].double().abs())
         assert_within(dB[g], ref, rounded(ref, err, torch.float32), f"dB {g}")
+    assert api.last_device_error() == 0
+
+
+# ------------------------------------------------------------------------------------------------ the largest sizes, and in place
+def test_most_groups_there_may_be(cuda_device):
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    G, N, K = 1024, 72, 136
+    sizes = [(7 * i * i) % 6 for i in range(G)]
+    bounds = [0]
+    for r in sizes:
+        bounds.append(bounds[-1] + r)
+    M = bounds[-1]
+    A, B, bias = make((M, K), F16, cuda_device, 1), make((G, N, K), F16, cuda_device, 2, K ** -0.5), make((G, N), F16, cuda_device, 3)
+    dC = make((M, N), F16, cuda_device, 4)
+    C, dA, dB = torch.empty_like(dC), torch.empty_like(A), torch.full((G, N, K), SENTINEL, device=cuda_device)
+    dbias = torch.full((G, N), SENTINEL, device=cuda_device)
+    offsets = torch.tensor(bounds, dtype=torch.int32, device=cuda_device)
+    api.hgemm_grouped(A, B, C, offsets, bias=bias, act="silu")
+    api.hgemm_grouped_backward(dC, A, B, offsets, dA=dA, dB=dB, dbias=dbias)
+    for g in range(G):
+        r = slice(bounds[g], bounds[g + 1])
+        if sizes[g]:
+            check_forward(A[r], B[g], bias[g], None, "silu", C[r], None, f"group {g}")
+            check_backward(dC[r], A[r], B[g], "none", None, None, dA[r], dB[g], dbias[g], f"group {g}")
+        else:
+            assert (dB[g] == 0).all() and (dbias[g] == 0).all()
+    assert api.last_device_error() == 0
+
+
+def test_a_stack_of_more_than_2_to_the_32_weights(cuda_device, most_memory):
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    G, N, K = 272, 4096, 4096  # 4.6e9 weights
+    if most_memory < 24:
+        pytest.skip("not enough free memory")
+    B = torch.zeros((G, N, K), dtype=torch.bfloat16, device=cuda_device)
+    last = (0, 255, 256, G - 1)  # around element 2^32, and the ends
+    for g in last:
+        B[g] = make((N, K), BF16, cuda_device, g, K ** -0.5)
+    A, dC = make((4 * G, K), BF16, cuda_device, 1), make((4 * G, N), BF16, cuda_device, 2)
+    offsets = torch.arange(0, 4 * G + 1, 4, dtype=torch.int32, device=cuda_device)
+    C, dA, dB = torch.full_like(dC, SENTINEL), torch.full_like(A, SENTINEL), torch.full_like(B, SENTINEL)
+    api.hgemm_grouped(A, B, C, offsets)
+    api.hgemm_grouped_backward(dC, A, B, offsets, dA=dA, dB=dB)
+    for g in last:
+        r = slice(4 * g, 4 * g + 4)
+        check_forward(A[r], B[g], None, None, "none", C[r], None, f"group {g}")
+        check_backward(dC[r], A[r], B[g], "none", None, None, dA[r], dB[g], None, f"group {g}")
+    assert (C[8:4 * 255] == 0).all() and (dA[8:4 * 255] == 0).all()
+    assert api.last_device_error() == 0
+
+
+def test_nearly_2_to_the_31_rows(cuda_device, most_memory):
+    """The most rows a call takes, 2^31 - 256: the last of them, and nothing behind them."""
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    M, N, K = 0x7fffff00, 8, 8
+    if most_memory < 110:
+        pytest.skip("not enough free memory")
+    A = torch.zeros((M, K), dtype=torch.float16, device=cuda_device)
+    A[-700:] = make((700, K), F16, cuda_device, 1)
+    B = make((2, N, K), F16, cuda_device, 2)
+    room = torch.full((M + 64, N), SENTINEL, dtype=torch.float16, device=cuda_device)
+    C = room[:M]
+    last = slice(M - 700, M)
+    api.hgemm_linear(A, B[0], C, act="relu")
+    check_forward(A[last], B[0], None, None, "relu", C[last], None, "linear")
+    offsets = torch.tensor([0, 5, M], dtype=torch.int32, device=cuda_device)
+    api.hgemm_grouped(A, B, C, offsets)
+    check_forward(A[last], B[1], None, None, "none", C[last], None, "grouped")
+    assert (room[M:] == SENTINEL).all()
+    # (a weight gradient of one group of so many rows is one tile's sum, which takes seconds; the linear layer's is cut into slices)
+    dA, dB, dbias = torch.full((M + 64, K), SENTINEL, dtype=torch.float16, device=cuda_device), torch.empty((N, K), device=cuda_device), torch.empty(N, device=cuda_device)
+    api.hgemm_grouped_backward(C, A, B, offsets, dA=dA[:M])
+    check_backward(C[last], A[last], B[1], "none", None, None, dA[:M][last], None, None, "grouped")
+    assert (dA[M:] == SENTINEL).all()
+    api.hgemm_linear_backward(C, A, B[1], dA=dA[:M], dB=dB, dbias=dbias)
+    check_backward(C[last], A[last], B[1], "none", None, None, dA[:M][last], dB, dbias, "linear")
+    assert api.last_device_error() == 0
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 72), (64, 1024, 8192), (16, 4096, 4096), (300, 701, 200), (777, 1000, 1544), (2000, 4096, 128)], ids=str)
+@pytest.mark.parametrize("dtype,out", [(F16, F16), (BF16, F32)])
+def test_residual_in_place_on_every_kernel(cuda_device, shape, dtype, out):
+    import torch
+
+    from cuda_hgemm_b200 import api
+
+    M, N, K = shape
+    A, B = make((M, K), dtype, cuda_device, 1), make((N, K), dtype, cuda_device, 2, K ** -0.5)
+    C = make((M, N), out, cuda_device, 3)
+    was, pre = C.clone(), torch.empty_like(C)
+    api.hgemm_linear(A, B, C, residual=C, act="gelu_tanh", pre=pre)
+    check_forward(A, B, None, was, "gelu_tanh", C, pre, "in place")
     assert api.last_device_error() == 0
