@@ -984,8 +984,12 @@ static int add_early_start(cudaLaunchAttribute *attr, bool early) {
     if (!early) return 0;
     attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr->val.programmaticStreamSerializationAllowed = 1;
-    g_early_skinny_launches.fetch_add(1, std::memory_order_relaxed);
     return 1;
+}
+
+static void count_skinny_launch(bool early) {
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (early) g_early_skinny_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
 static std::atomic<int> g_debug_cluster_capacity{0};  // b200_debug_cluster_capacity(): > 0 overrides what the device reports
@@ -1065,7 +1069,7 @@ static int launch_skinny_kernel(DeviceState &st, int attr_slot, const SkinnyPara
         cudaGetLastError();
         return B200_HGEMM_ERR_CUDA;
     }
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+    count_skinny_launch(!p.after_all);
     return B200_HGEMM_OK;
 }
 
@@ -1162,7 +1166,7 @@ static int run_skinny(DeviceState &st, const void *A, const void *B, void *C, si
         cudaGetLastError();
         return B200_HGEMM_ERR_CUDA;
     }
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+    count_skinny_launch(start.early);
     return B200_HGEMM_OK;
 }
 
